@@ -16,6 +16,7 @@ HEADER = PKG.parent / "include" / "g4w4.h"
 
 G4_OK = 0
 G4_ROWS_HISTORY_READY = 1
+G4_TREE_MAX_NODES = 64
 G4_F32 = 0
 G4_BF16 = 1
 
@@ -29,6 +30,18 @@ class G4Rows(C.Structure):
 class G4Planes(C.Structure):
     """g4_planes: a linear's f32 output as partial planes summed in slice order (include/g4w4.h)."""
     _fields_ = [("base", C.c_void_p), ("count", C.c_int), ("stride", C.c_longlong), ("ld", C.c_int)]
+
+
+class G4Sampling(C.Structure):
+    """g4_sampling: per-row device arrays of the sampling settings (include/g4w4.h)."""
+    _fields_ = [("temperature", C.c_void_p), ("top_k", C.c_void_p), ("top_p", C.c_void_p), ("min_p", C.c_void_p),
+                ("uniform", C.c_void_p)]
+
+
+class G4Tree(C.Structure):
+    """g4_tree: the drafted tokens' tree of each sequence (include/g4w4.h)."""
+    _fields_ = [("parents", C.c_void_p), ("parent_stride", C.c_int), ("nodes", C.c_int), ("counts", C.c_void_p)]
+
 
 class G4DecoderLayer(C.Structure):
     """g4_decoder_layer (include/g4w4.h)."""
@@ -129,6 +142,13 @@ SIGNATURES = {
     "g4_ple_mix": (_S, [_P, _P, _F, _P, _P, _I, _I, _I, _F, _P]),
     "g4_softcap_argmax": (_S, [_P, _P, _I, _I, _F, _P, _P]),
     "g4_advance_positions": (_S, [_P, _P, _I, _I, _I]),
+    "g4_sample": (_S, [_P, _P, C.c_longlong, _I, _I, _F, _P, _P, _P]),
+    "g4_attention_tree": (_S, [_P, _P, _P, _I, _I, _I, _P, _P, _I, _I, _I, _P]),
+    "g4_qkv_post_tree": (_S, [_P, _P, _I, _I, _P, _P, _F, _I, _F, _P, _P, _I, _P, _P, _I]),
+    "g4_tree_accept": (_S, [_P, _P, _I, _P, _P, _P, _P, _P]),
+    "g4_kv_compact": (_S, [_P, _P, _I, _I, _P, _I, _I, _I, _P, _P]),
+    "g4_kv_fork": (_S, [_P, _P, _I, _I, _P, _P, _P, _I]),
+    "g4_advance_positions_each": (_S, [_P, _P, _I, _I, _P]),
     "g4_dense_create": (_S, [_P, _P, _I, _I, _I, _PP]),
     "g4_dense_destroy": (_S, [_P]),
     "g4_dense_weights": (_S, [_P, _PP]),

@@ -16,6 +16,7 @@
 #include "g4_attention.cuh"
 #include "g4_common.cuh"
 #include "g4_glue.cuh"
+#include "g4_tree.cuh"
 
 namespace {
 
@@ -295,22 +296,35 @@ __device__ __forceinline__ float2 qkv_pair(int slot, int H, int hd, int i, float
                       rope_angles, rope_base, pos);
 }
 
+// kTree: rows are nodes of drafted trees: K/V go to the row's position as above, the rotation
+// is that of base + depth, and rows behind their sequence's count are skipped.
+
 // Any hd % 64 == 0: one CTA per (row, head slot), thread i owns the rotation pair
 // (i, i + hd/2).
+template <bool kTree>
 __global__ void qkv_post_kernel(Planes y, int H, int hd, int has_kv,
                                 const float* __restrict__ qnorm, const float* __restrict__ knorm, float eps,
-                                int rope_angles, float rope_base, G4Rows R, uint16_t* __restrict__ q_out, KvSink kv) {
+                                int rope_angles, float rope_base, G4Rows R, uint16_t* __restrict__ q_out, KvSink kv,
+                                g4_tree tree) {
     pdl_trigger();
     pdl_wait();
     __shared__ float red[32];
-    const int slot = blockIdx.x, r = blockIdx.y;
+    const int slot = blockIdx.x, r = kTree ? blockIdx.y + gridDim.y * blockIdx.z : blockIdx.y;
+    int depth = 0;
+    if (kTree) {
+        const int s = r / R.rows_per_seq, node = r - s * R.rows_per_seq;
+        const int count = tree_count(tree, s, kv.err);
+        if (node >= count) return;  // the whole CTA
+        depth = warp_tree_depth(load_warp_tree(tree, s, count, kv.err), node);
+    }
     const int half = hd >> 1;
     const int i = threadIdx.x;  // 0 .. half-1
     const size_t src = (size_t)r * y.ld + (size_t)slot * hd;
     const float a0 = ld_planes(y, src + i), a1 = ld_planes(y, src + i + half);
     const float inv = rsqrtf(block_sum(a0 * a0 + a1 * a1, red) / (float)hd + eps);
     const int pos = row_position(R, r);
-    const float2 o = qkv_pair(slot, H, hd, i, a0, a1, inv, qnorm, knorm, rope_angles, rope_base, pos);
+    const int rot = kTree ? pos - r % R.rows_per_seq + depth : pos;
+    const float2 o = qkv_pair(slot, H, hd, i, a0, a1, inv, qnorm, knorm, rope_angles, rope_base, rot);
     if (!kv_row_ok(slot, H, pos, kv)) return;
     uint16_t* dst2;
     uint16_t* dst = qkv_dst(slot, H, hd, r, R, pos, q_out, kv, &dst2);
@@ -329,11 +343,11 @@ __global__ void qkv_post_kernel(Planes y, int H, int hd, int has_kv,
 // 4 NF rotation pairs.  The planes are summed in slice order with the loads of a batch
 // of slices for all the lane's groups in flight together.
 constexpr int kQkvWarps = 8;
-template <int NF>
+template <int NF, bool kTree>
 __global__ void __launch_bounds__(kQkvWarps * 32)
 qkv_post_warp_kernel(Planes y, int H, int has_kv, int rows, const float* __restrict__ qnorm,
                      const float* __restrict__ knorm, float eps, int rope_angles, float rope_base, G4Rows R,
-                     uint16_t* __restrict__ q_out, KvSink kv) {
+                     uint16_t* __restrict__ q_out, KvSink kv, g4_tree tree) {
     constexpr int hd = 256 * NF, half = hd / 2, G = 2 * NF;  // float4 groups per lane
     constexpr int PB = NF <= 2 ? 4 : 2;                        // slices per load batch
     pdl_trigger();
@@ -358,6 +372,13 @@ qkv_post_warp_kernel(Planes y, int H, int has_kv, int rows, const float* __restr
     if (!valid) return;
     const int seq = row_seq(R, r);
     const int seq_pos = R.seq_pos ? R.seq_pos[seq] : 0;
+    WarpTree wt{-1, -1};
+    if (kTree) {
+        const int s = r / R.rows_per_seq;
+        const int count = tree_count(tree, s, kv.err);
+        if (r - s * R.rows_per_seq >= count) return;
+        wt = load_warp_tree(tree, s, count, kv.err);
+    }
     const float* src = y.base + (size_t)r * y.ld + (size_t)slot * hd;
     float4 a[G];
 #pragma unroll
@@ -391,6 +412,7 @@ qkv_post_warp_kernel(Planes y, int H, int has_kv, int rows, const float* __restr
     for (int off = 16; off > 0; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
     const float inv = rsqrtf(ss / (float)hd + eps);
     const int pos = seq_pos + R.pos0 + r % R.rows_per_seq;
+    const int rot = kTree ? seq_pos + R.pos0 + warp_tree_depth(wt, r % R.rows_per_seq) : pos;
     if (!kv_row_ok(slot, H, pos, kv)) return;
     uint16_t* dst2;
     uint16_t* dst = qkv_dst(slot, H, hd, r, R, pos, q_out, kv, &dst2);
@@ -404,7 +426,7 @@ qkv_post_warp_kernel(Planes y, int H, int has_kv, int rows, const float* __restr
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
             const float2 o = qkv_pair_s(slot, H, hd, i0 + c, lo[c], hi[c], inv, slo[c], shi[c], rope_angles, rope_base,
-                                        pos);
+                                        rot);
             o0[c] = o.x;
             o1[c] = o.y;
         }
@@ -539,6 +561,14 @@ __global__ void __launch_bounds__(256) argmax_final_kernel(const float2* __restr
         ids[r] = si[0];
         if (vals) vals[r] = sv[0];
     }
+}
+
+// Advances the position of sequence seq_base + i by by[i].
+__global__ void advance_pos_each_kernel(int32_t* seq_pos, int seq_base, int nseq, const int32_t* __restrict__ by) {
+    pdl_trigger();
+    pdl_wait();
+    const int i = blockIdx.x * blockDim.x + threadIdx.x;
+    if (i < nseq) seq_pos[seq_base + i] += by[i];
 }
 
 // Advances the positions of sequences [seq_base, seq_base + nseq) by `by`.
@@ -689,7 +719,7 @@ namespace {
 g4_status qkv_post_impl(g4_ctx* ctx, const g4_planes* y, int heads, int hd, int has_kv, const float* qnorm,
                         const float* knorm, float eps, int rope_angles, float rope_base, const G4Rows* rows_map,
                         int rows, void* q_out_bf16, void* kcache_bf16, void* vcache_bf16, int cache_cap, int ring,
-                        int mirror, int pos_limit) {
+                        int mirror, int pos_limit, const g4_tree* tree = nullptr) {
     g4_status st = g4::use_device(ctx);
     if (st) return st;
     if (rows < 0 || !planes_ok(y) || !qnorm || !rows_map || !q_out_bf16 ||
@@ -707,14 +737,19 @@ g4_status qkv_post_impl(g4_ctx* ctx, const g4_planes* y, int heads, int hd, int 
     uint16_t* qo = static_cast<uint16_t*>(q_out_bf16);
     const KvSink kv{static_cast<uint16_t*>(kcache_bf16), static_cast<uint16_t*>(vcache_bf16), cache_cap, ring, mirror,
                     pos_limit, ctx->d_err};
+    const g4_tree t = tree ? *tree : g4_tree{};
     if (f4 && hd == 256)
-        return g4::launch(ctx, "qkv_post_warp_kernel", qkv_post_warp_kernel<1>, wgrid, wblock, 0, 1, P, heads, has_kv,
-                          rows, qnorm, knorm, eps, rope_angles, rope_base, *rows_map, qo, kv);
+        return g4::launch(ctx, "qkv_post_warp_kernel", tree ? qkv_post_warp_kernel<1, true> : qkv_post_warp_kernel<1, false>,
+                          wgrid, wblock, 0, 1, P, heads, has_kv, rows, qnorm, knorm, eps, rope_angles, rope_base, *rows_map,
+                          qo, kv, t);
     if (f4 && hd == 512)
-        return g4::launch(ctx, "qkv_post_warp_kernel", qkv_post_warp_kernel<2>, wgrid, wblock, 0, 1, P, heads, has_kv,
-                          rows, qnorm, knorm, eps, rope_angles, rope_base, *rows_map, qo, kv);
-    return g4::launch(ctx, "qkv_post_kernel", qkv_post_kernel, dim3(heads + (has_kv ? 2 : 0), rows), dim3(hd / 2), 0,
-                      1, P, heads, hd, has_kv, qnorm, knorm, eps, rope_angles, rope_base, *rows_map, qo, kv);
+        return g4::launch(ctx, "qkv_post_warp_kernel", tree ? qkv_post_warp_kernel<2, true> : qkv_post_warp_kernel<2, false>,
+                          wgrid, wblock, 0, 1, P, heads, has_kv, rows, qnorm, knorm, eps, rope_angles, rope_base, *rows_map,
+                          qo, kv, t);
+    const dim3 grid = tree ? dim3(heads + (has_kv ? 2 : 0), tree->nodes, rows / tree->nodes)
+                           : dim3(heads + (has_kv ? 2 : 0), rows);
+    return g4::launch(ctx, "qkv_post_kernel", tree ? qkv_post_kernel<true> : qkv_post_kernel<false>, grid, dim3(hd / 2), 0,
+                      1, P, heads, hd, has_kv, qnorm, knorm, eps, rope_angles, rope_base, *rows_map, qo, kv, t);
 }
 
 }  // namespace
@@ -743,6 +778,26 @@ g4_status g4_qkv_post_kv(g4_ctx* ctx, const g4_planes* y, int heads, int hd, con
         return g4::set_error(G4_ERR_RANGE, "g4_qkv_post_kv: sequences beyond the cache (%d rows)", kv->rows_total);
     return qkv_post_impl(ctx, y, heads, hd, 1, qnorm, knorm, eps, rope_angles, rope_base, rows_map, rows, q_out_bf16,
                          kv->k, kv->v, seq_rows, kv->ring, kv->mirror, kv->ring ? kv->capacity : seq_rows);
+}
+
+g4_status g4_qkv_post_tree(g4_ctx* ctx, const g4_planes* y, int heads, int hd, const float* qnorm, const float* knorm,
+                           float eps, int rope_angles, float rope_base, const G4Rows* rows_map, const g4_tree* tree,
+                           int rows, void* q_out_bf16, const g4_kv* kv, int seq_stride) {
+    const g4_status st = g4::check_tree_rows("g4_qkv_post_tree", rows_map, tree, rows);
+    if (st) return st;
+    if (heads < 1) return g4::set_error(G4_ERR_INVALID, "g4_qkv_post_tree: %d heads", heads);
+    if (rows / tree->nodes > 65535)
+        return g4::set_error(G4_ERR_UNSUPPORTED, "g4_qkv_post_tree: %d sequences (65535 supported)", rows / tree->nodes);
+    if (!kv)
+        return qkv_post_impl(ctx, y, heads, hd, 0, qnorm, knorm, eps, rope_angles, rope_base, rows_map, rows,
+                             q_out_bf16, nullptr, nullptr, 1, 0, 0, 1, tree);
+    if (hd != kv->hd) return g4::set_error(G4_ERR_INVALID, "g4_qkv_post_tree: hd %d != cache hd %d", hd, kv->hd);
+    const int seq_rows = kv->ring ? kv->seq_rows : seq_stride;
+    if (seq_rows < 1) return g4::set_error(G4_ERR_INVALID, "g4_qkv_post_tree: seq_stride %d", seq_stride);
+    if ((long long)(rows_map->seq_base + (long long)rows / tree->nodes) * seq_rows > kv->rows_total)
+        return g4::set_error(G4_ERR_RANGE, "g4_qkv_post_tree: sequences beyond the cache (%d rows)", kv->rows_total);
+    return qkv_post_impl(ctx, y, heads, hd, 1, qnorm, knorm, eps, rope_angles, rope_base, rows_map, rows, q_out_bf16,
+                         kv->k, kv->v, seq_rows, kv->ring, kv->mirror, kv->ring ? kv->capacity : seq_rows, tree);
 }
 
 g4_status g4_qkv_post(g4_ctx* ctx, const float* y, int ldy, int heads, int hd, int has_kv, const float* qnorm,
@@ -883,6 +938,15 @@ g4_status g4_advance_positions(g4_ctx* ctx, int32_t* seq_pos, int seq_base, int 
     if (nseq == 0) return G4_OK;
     return g4::launch(ctx, "advance_pos_kernel", advance_pos_kernel, dim3(blocks_for(nseq, 256)), dim3(256), 0, 1,
                       seq_pos, seq_base, nseq, by);
+}
+
+g4_status g4_advance_positions_each(g4_ctx* ctx, int32_t* seq_pos, int seq_base, int nseq, const int32_t* by) {
+    if (!seq_pos || !by || nseq < 0 || seq_base < 0)
+        return g4::set_error(G4_ERR_INVALID, "g4_advance_positions_each: bad arguments");
+    const g4_status st = g4::use_device(ctx);
+    if (st || nseq == 0) return st;
+    return g4::launch(ctx, "advance_pos_each_kernel", advance_pos_each_kernel, dim3(blocks_for(nseq, 256)), dim3(256), 0,
+                      1, seq_pos, seq_base, nseq, by);
 }
 
 }  // extern "C"

@@ -16,7 +16,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from ._lib import G4_BF16, G4_F32, G4Error, call
+from ._lib import G4_BF16, G4_F32, G4Error, G4Rows, G4Sampling, G4Tree, call
 
 _DT = {torch.float32: G4_F32, torch.bfloat16: G4_BF16}
 
@@ -32,6 +32,16 @@ def _host_or_device(a) -> tuple[C.c_void_p, int, object]:
         return C.c_void_p(a.data_ptr()), int(a.is_cuda), a
     a = np.ascontiguousarray(a)
     return C.c_void_p(a.ctypes.data), 0, a
+
+
+def _need(ctx: "Context", name: str, what: str, t: torch.Tensor, dtype: torch.dtype, shape: tuple | None = None) -> int:
+    """The device pointer of a contiguous tensor argument of the context's device, type and shape."""
+    if t.dtype != dtype or not t.is_cuda or t.device != ctx.torch_device or not t.is_contiguous() or (
+            shape is not None and tuple(t.shape) != shape):
+        raise G4Error(-1, f"{name}: {what} must be a contiguous {dtype} tensor"
+                          f"{'' if shape is None else f' of shape {shape}'} on {ctx.torch_device}, got {t.dtype} "
+                          f"{tuple(t.shape)} with strides {tuple(t.stride())} on {t.device}")
+    return t.data_ptr()
 
 
 class Context:
@@ -61,6 +71,24 @@ class Context:
 
     def sync(self) -> None:
         call("g4_stream_sync", self.handle)
+
+    def empty(self, shape, dtype: torch.dtype, *used: torch.Tensor | None) -> torch.Tensor:
+        """An output tensor of a call on this context's stream.  When that is not torch's current
+        stream, the output comes from the context stream's own memory (a block that torch still
+        uses elsewhere cannot be handed out early), and the call's inputs (`used`) are not reused
+        before the context stream is done with them."""
+        if torch.cuda.current_stream(self.torch_device) == self._stream:
+            return torch.empty(shape, dtype=dtype, device=self.torch_device)
+        for t in used:
+            if t is not None:
+                t.record_stream(self._stream)
+        with torch.cuda.stream(self._stream):
+            return torch.empty(shape, dtype=dtype, device=self.torch_device)
+
+    def fill(self, t: torch.Tensor, value) -> None:
+        """t.fill_(value) on the context's stream."""
+        with torch.cuda.stream(self._stream):
+            t.fill_(value)
 
     def check_device(self) -> int:
         """Raises G4Error if a kernel raised the device error word since the last check."""
@@ -219,6 +247,14 @@ class KVCache:
     def reset(self) -> None:
         call("g4_kv_reset", self.handle)
 
+    def storage(self) -> tuple[torch.Tensor, torch.Tensor]:
+        """The bf16 K and V storage [rows, head_dim] itself, as tensors that share its memory
+        and keep the cache alive.  The library reads and writes it on the context's stream."""
+        kp, vp = C.c_void_p(), C.c_void_p()
+        call("g4_kv_buffers", self.handle, C.byref(kp), C.byref(vp))
+        return tuple(torch.as_tensor(_Storage(self, p.value), device=self.ctx.torch_device).view(torch.bfloat16)
+                     for p in (kp, vp))
+
     def tensors(self) -> tuple[torch.Tensor, torch.Tensor]:
         """Copies of the bf16 K and V storage [rows, head_dim] (for tests)."""
         kp, vp = C.c_void_p(), C.c_void_p()
@@ -237,6 +273,53 @@ class KVCache:
             self.close()
         except Exception:
             pass
+
+
+class _Storage:
+    """A cache's K or V storage for torch.as_tensor (no copy; the tensor keeps this object)."""
+
+    def __init__(self, cache: KVCache, ptr: int):
+        self.cache = cache
+        self.__cuda_array_interface__ = {"shape": (cache.rows, cache.head_dim), "typestr": "<i2", "strides": None,
+                                         "data": (ptr, False), "version": 2}
+
+
+def _cache_table(caches) -> C.Array:
+    return (C.c_void_p * len(caches))(*[c.handle for c in caches])
+
+
+def _seq_stride(caches, seq_stride: int | None) -> int:
+    """Rows per sequence of the linear caches (a ring cache has its own): all of them by default."""
+    return seq_stride or min((c.rows for c in caches if not c.ring), default=1)
+
+
+def kv_compact(ctx: Context, caches, seq_pos: torch.Tensor, path: torch.Tensor, accepted: torch.Tensor,
+               seq_stride: int | None = None, seq_base: int = 0) -> None:
+    """Moves the accepted rows of drafted trees together behind the cached ones, in every cache of
+    the list at once (g4_kv_compact): path int32 [nseq, nodes] and accepted int32 [nseq] as
+    GPUOps.treeAccept returns them, seq_pos the int32 positions before the drafted tokens."""
+    nseq, nodes = path.shape
+    pp = _need(ctx, "kv_compact", "path", path, torch.int32)
+    ap = _need(ctx, "kv_compact", "accepted", accepted, torch.int32, (nseq,))
+    sp = _need(ctx, "kv_compact", "seq_pos", seq_pos, torch.int32)
+    if seq_base < 0 or seq_base + nseq > seq_pos.numel():
+        raise G4Error(-6, f"kv_compact: sequences {seq_base}..{seq_base + nseq} of {seq_pos.numel()} positions")
+    call("g4_kv_compact", ctx.handle, _cache_table(caches), len(caches), _seq_stride(caches, seq_stride), sp, seq_base,
+         nseq, nodes, pp, ap)
+
+
+def kv_fork(ctx: Context, caches, seq_pos: torch.Tensor, src, dst, seq_stride: int | None = None) -> None:
+    """Copies the cached rows and the position of sequence src[i] to sequence dst[i], in every cache
+    of the list at once (g4_kv_fork); src and dst are sequences of ints on the host."""
+    src, dst = [int(i) for i in src], [int(i) for i in dst]
+    if len(src) != len(dst):
+        raise G4Error(-1, f"kv_fork: {len(src)} sources, {len(dst)} destinations")
+    sp = _need(ctx, "kv_fork", "seq_pos", seq_pos, torch.int32)
+    n = len(src)
+    if any(not 0 <= i < seq_pos.numel() for i in (*src, *dst)):
+        raise G4Error(-6, f"kv_fork: sequences {src} -> {dst} of {seq_pos.numel()} positions")
+    call("g4_kv_fork", ctx.handle, _cache_table(caches), len(caches), _seq_stride(caches, seq_stride), sp,
+         (C.c_int32 * n)(*src), (C.c_int32 * n)(*dst), n)
 
 
 def _wrap_device(ptr: int, n: int, ctx: Context) -> torch.Tensor:
@@ -367,6 +450,81 @@ class GPUOps:
         call("g4_ple_mix", self.ctx.handle, _ptr(proj), C.c_float(1.0), _ptr(normScale), _ptr(tokenPle), rows,
              layers, dim, C.c_float(1e-6), _ptr(y))
         return y
+
+
+    # ---- sampling and drafted trees (no counterpart in the reference, which answers greedily) ----
+    def sample(self, logits: torch.Tensor, uniform: torch.Tensor, temperature: torch.Tensor | None = None,
+               top_k: torch.Tensor | None = None, top_p: torch.Tensor | None = None, min_p: torch.Tensor | None = None,
+               cap: float = 0.0) -> tuple[torch.Tensor, torch.Tensor]:
+        """One token per row of f32 logits [rows, vocab] (rows may be strided) from one uniform
+        number per row: (ids int32 [rows], probs f32 [rows]) of g4_sample.  The settings are
+        device tensors of one entry per row (f32; top_k int32), None = off."""
+        if logits.dtype != torch.float32 or logits.dim() != 2 or logits.device != self.ctx.torch_device or (
+                logits.shape[1] > 1 and logits.stride(1) != 1):
+            raise G4Error(-1, f"sample: logits must be f32 [rows, vocab] rows on {self.ctx.torch_device}, got "
+                              f"{logits.dtype} {tuple(logits.shape)} strides {logits.stride()} on {logits.device}")
+        rows, vocab = logits.shape
+        ld = logits.stride(0) if rows > 1 else vocab
+
+        def arg(what, t, dtype=torch.float32):
+            return None if t is None else _need(self.ctx, "sample", what, t, dtype, (rows,))
+
+        how = G4Sampling(arg("temperature", temperature), arg("top_k", top_k, torch.int32), arg("top_p", top_p),
+                         arg("min_p", min_p), arg("uniform", uniform))
+        ids = self.ctx.empty(rows, torch.int32, logits, uniform, temperature, top_k, top_p, min_p)
+        probs = self.ctx.empty(rows, torch.float32)
+        call("g4_sample", self.ctx.handle, _ptr(logits), ld, rows, vocab, C.c_float(cap), C.byref(how), _ptr(ids),
+             _ptr(probs))
+        return ids, probs
+
+    def _tree(self, name: str, parents: torch.Tensor, nseq: int, nodes: int, counts: torch.Tensor | None) -> G4Tree:
+        shared = parents.dim() == 1
+        pp = _need(self.ctx, name, "parents", parents, torch.int32, (nodes,) if shared else (nseq, nodes))
+        return G4Tree(pp, 0 if shared else nodes, nodes,
+                      None if counts is None else _need(self.ctx, name, "counts", counts, torch.int32, (nseq,)))
+
+    def attentionTree(self, q: torch.Tensor, cache: KVCache, seq_pos: torch.Tensor, parents: torch.Tensor,  # noqa: N802
+                      counts: torch.Tensor | None = None, seq_stride: int | None = None, seq_base: int = 0,
+                      sliding: bool = False, window: int = 0, out: torch.Tensor | None = None) -> torch.Tensor:
+        """Attention of drafted trees (g4_attention_tree): q bf16 [nseq, nodes, heads, hd], the
+        drafted rows' K/V already in the cache at seq_pos + node; parents int32 [nseq, nodes], or
+        [nodes] for one tree of all sequences.  Rows behind a sequence's count keep what `out`
+        held (0 in a new one)."""
+        if q.dim() != 4:
+            raise G4Error(-1, f"attentionTree: q must be [nseq, nodes, heads, hd], got {tuple(q.shape)}")
+        nseq, nodes, heads, hd = q.shape
+        qp = _need(self.ctx, "attentionTree", "q", q, torch.bfloat16)
+        sp = _need(self.ctx, "attentionTree", "seq_pos", seq_pos, torch.int32)
+        if seq_base < 0 or seq_base + nseq > seq_pos.numel():
+            raise G4Error(-6, f"attentionTree: sequences {seq_base}..{seq_base + nseq} of {seq_pos.numel()} positions")
+        tree = self._tree("attentionTree", parents, nseq, nodes, counts)
+        if out is None:
+            out = self.ctx.empty(q.shape, torch.bfloat16, q, seq_pos, parents, counts)
+            if counts is not None:  # rows that no node writes
+                self.ctx.fill(out, 0)
+        op = _need(self.ctx, "attentionTree", "out", out, torch.bfloat16, tuple(q.shape))
+        rmap = G4Rows(sp, seq_base, nodes, 0, 0)
+        call("g4_attention_tree", self.ctx.handle, qp, cache.handle, nseq * nodes, heads, hd, C.byref(rmap),
+             C.byref(tree), cache.seq_rows if cache.ring else _seq_stride([cache], seq_stride), int(bool(sliding)), window,
+             op)
+        return out
+
+    def treeAccept(self, parents: torch.Tensor, tokens: torch.Tensor, picks: torch.Tensor,  # noqa: N802
+                   counts: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        """The accepted path of each drafted tree (g4_tree_accept): tokens and picks int32
+        [nseq, nodes]; returns (path [nseq, nodes], accepted [nseq], next [nseq]), int32 (next is
+        -1 for a sequence without nodes)."""
+        nseq, nodes = tokens.shape
+        tp = _need(self.ctx, "treeAccept", "tokens", tokens, torch.int32)
+        kp = _need(self.ctx, "treeAccept", "picks", picks, torch.int32, (nseq, nodes))
+        tree = self._tree("treeAccept", parents, nseq, nodes, counts)
+        path = self.ctx.empty((nseq, nodes), torch.int32, parents, tokens, picks, counts)
+        accepted = self.ctx.empty(nseq, torch.int32)
+        nxt = self.ctx.empty(nseq, torch.int32)
+        if counts is not None:
+            self.ctx.fill(nxt, -1)
+        call("g4_tree_accept", self.ctx.handle, C.byref(tree), nseq, tp, kp, _ptr(path), _ptr(accepted), _ptr(nxt))
+        return path, accepted, nxt
 
 
 def launch_count() -> int:

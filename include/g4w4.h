@@ -357,6 +357,97 @@ g4_status g4_softcap_argmax(g4_ctx* ctx, const float* logits, int rows, int voca
 /* seq_pos[seq_base .. seq_base + nseq) += by (device-side step counter of a decode loop). */
 g4_status g4_advance_positions(g4_ctx* ctx, int32_t* seq_pos, int seq_base, int nseq, int by);
 
+/* --------------------------------------------------------------- sampling --
+ * The reference answers greedily (topK :1396-1425, gemma4-webgpu.js:465-478); these are the
+ * usual settings of a sampled answer, each a device array of one entry per row (so a captured
+ * step replays with other settings), or NULL for "off". */
+typedef struct {
+    const float* temperature;  /* NULL: 1.  Not > 0 (or NaN): the row's greedy pick              */
+    const int32_t* top_k;      /* < 1 or >= vocab: off                                          */
+    const float* top_p;        /* >= 1 (or NaN): off; <= 0: the highest logit alone             */
+    const float* min_p;        /* <= 0 (or NaN): off; >= 1: only logits equal to the highest    */
+    const float* uniform;      /* required: the row's random number in [0, 1) (others clamped)  */
+} g4_sampling;
+/* One token per row of f32 logits [rows, ld] (ld >= vocab).  With cap > 0 the logits are first
+ * capped as g4_softcap does (the same bits as g4_softcap in place, then this call with cap 0).
+ * NaN and -inf logits are never picked.  The others are ranked by (logit descending, index
+ * ascending) and weigh w = exp((logit - highest) / temperature); +inf logits share the whole
+ * weight.  Kept is a prefix of the ranking, the shortest of
+ *   top_k ranks;  the shortest prefix of those that holds top_p of their weight;  the ranks
+ *   with w >= min_p.
+ * ids_out[r] is the lowest index i whose kept weights up to and with i, in index order, sum to
+ * more than uniform[r] times the kept weight; probs_out[r] (may be NULL) its share of the kept
+ * weight (1 for a greedy row).  A row with nothing to pick gives -1 and 0.  Weights and sums
+ * are held in 64 bits, in an order that does not depend on the launch.
+ * vocab at most 786432 (G4_ERR_UNSUPPORTED). */
+g4_status g4_sample(g4_ctx* ctx, const float* logits, long long ld, int rows, int vocab, float cap,
+                    const g4_sampling* how, int32_t* ids_out, float* probs_out);
+
+/* -------------------------------------------------- trees of drafted tokens --
+ * No reference counterpart: the reference decodes one token per step.  A tree holds `nodes`
+ * drafted tokens of each sequence.  Node i hangs under node parents[s * parent_stride + i] < i
+ * of its sequence, or directly behind the cached tokens (-1); its depth is the number of its
+ * ancestors.  parent_stride 0 gives every sequence the same tree.  counts (may be NULL) says
+ * how many nodes of each sequence are used; rows behind them are neither read nor written.
+ * s counts the sequences of the call (row / nodes), not of the cache.  A parent outside
+ * [-1, i) counts as -1 and raises G4_DEVERR_BAD_INDEX; so does a count outside [0, nodes],
+ * which is clamped. */
+#define G4_TREE_MAX_NODES 64
+typedef struct {
+    const int32_t* parents;
+    int parent_stride;
+    int nodes;
+    const int32_t* counts;
+} g4_tree;
+/* g4_attention_rows for drafted trees.  The rows map gives the sequences: rows_per_seq =
+ * tree->nodes, and base = seq_pos[seq] + pos0 cached rows before the drafted ones.  The K/V of
+ * node i sit at position base + i (g4_qkv_post_tree), its query at position base + depth.
+ * Row (s, i) sees the cached keys j < base and, of the drafted ones, its ancestors and itself;
+ * when sliding, only keys less than `window` positions before its own (a drafted key's position
+ * is base + its depth).  q, out: bf16 [rows, heads, hd], rows a multiple of nodes; logit scale
+ * 1.0; heads 1..8, hd in {64,128,256,512}, q and out 16-byte aligned.  What masked cache rows
+ * hold, NaN and infinity included, does not reach a row that does not see them; a row that sees
+ * a value row (V) that is not finite is NaN throughout.  A sequence whose drafted rows would
+ * not fit its seq_stride (or a ring cache's capacity) is left out and raises
+ * G4_DEVERR_BAD_INDEX.  Long key ranges are split over CTAs with partial results in the context
+ * workspace (as g4_attention_rows).  G4_ROWS_HISTORY_READY as for g4_attention_rows. */
+g4_status g4_attention_tree(g4_ctx* ctx, const void* q_bf16, const g4_kv* kv, int rows, int heads, int hd,
+                            const g4_rows* map, const g4_tree* tree, int seq_stride, int sliding, int window,
+                            void* out_bf16);
+/* g4_qkv_post_kv at tree positions: q and k of node i are rotated to position base + depth, K/V
+ * go to position base + i of the sequence's rows (seq * seq_stride, or a ring cache's own rows).
+ * kv = NULL processes q only.  Rows behind a sequence's count are skipped. */
+g4_status g4_qkv_post_tree(g4_ctx* ctx, const g4_planes* y, int heads, int hd, const float* qnorm, const float* knorm,
+                           float eps, int rope_angles, float rope_base, const g4_rows* map, const g4_tree* tree,
+                           int rows, void* q_out_bf16, const g4_kv* kv, int seq_stride);
+/* The accepted path of each sequence's tree, for trees whose node 0 is the sequence's current
+ * token (already chosen, so always accepted).  picks[s * nodes + i] is the model's token after
+ * node i (greedy or g4_sample), tokens[s * nodes + i] the drafted token at node i.  From node 0
+ * the walk goes to the lowest-numbered child that holds the pick of the node it is at, until
+ * there is none.  path_out[s * nodes + j] = the j-th node (entries behind the path: -1),
+ * accepted_out[s] = its length, next_out[s] = the pick after its last node.  A sequence with
+ * count 0 gets accepted 0 and keeps its next_out. */
+g4_status g4_tree_accept(g4_ctx* ctx, const g4_tree* tree, int nseq, const int32_t* tokens, const int32_t* picks,
+                         int32_t* path_out, int32_t* accepted_out, int32_t* next_out);
+/* Moves the K/V rows of an accepted path together, in every cache of a host array `kvs` (each
+ * cache once; linear caches with seq_stride rows per sequence, ring caches with their own):
+ * for j < accepted[s], position seq_pos[seq] + j <- position seq_pos[seq] + path[s * nodes + j],
+ * seq = seq_base + s.  path must rise strictly below `nodes` (g4_tree_accept's does): a sequence
+ * whose path does not, or whose drafted rows lie outside its cache, is left as it is and raises
+ * G4_DEVERR_BAD_INDEX.  Advance seq_pos afterwards (g4_advance_positions_each).  The length that
+ * g4_kv_append keeps is not touched. */
+g4_status g4_kv_compact(g4_ctx* ctx, g4_kv* const* kvs, int nkv, int seq_stride, const int32_t* seq_pos, int seq_base,
+                        int nseq, int nodes, const int32_t* path, const int32_t* accepted);
+/* Copies the cached rows of sequence src[i] to sequence dst[i], i < n (host arrays), in every
+ * cache of a host array `kvs`: the seq_pos[src] positions that the source holds (a ring cache's
+ * last ones), and seq_pos[dst] = seq_pos[src].  What the destinations held behind them stays.
+ * A destination may appear once and not among the sources (G4_ERR_INVALID).  A source position
+ * outside its cache raises G4_DEVERR_BAD_INDEX and copies nothing. */
+g4_status g4_kv_fork(g4_ctx* ctx, g4_kv* const* kvs, int nkv, int seq_stride, int32_t* seq_pos, const int32_t* src,
+                     const int32_t* dst, int n);
+/* seq_pos[seq_base + s] += by[s] for s < nseq (by on the device: the accepted counts). */
+g4_status g4_advance_positions_each(g4_ctx* ctx, int32_t* seq_pos, int seq_base, int nseq, const int32_t* by);
+
 /* ------------------------------------------------------- bf16 dense (LM head) --
  * The tied bf16 embedding used as the LM head (gemma4-webgpu.js:170-188, BF16_HEAD
  * :1265-1277): w bf16 [N, K], copied to the device (NULL w: allocate only). */

@@ -1,0 +1,252 @@
+"""Sampling from f32 logits (g4_sample) against the definition in 64 bits.
+
+Which token a row gives is a comparison of 64-bit sums of up to 786432 weights <= 1: both
+sides' sums are within 786432 * 2^-53 < 1e-10 of the real ones (relative to the kept weight), so
+ids have to be equal wherever no border lies within 1e-9 of the random number.  Probabilities
+are one rounding to f32 (2^-24) away from the quotient.
+"""
+import ctypes as C
+
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def reference(l, u, T=1.0, k=0, p=1.0, mp=0.0):
+    """(id, prob, distance of u to the next border, ids on both sides of it) of one f32 row."""
+    l = np.asarray(l, np.float32).astype(np.float64)
+    V = l.size
+    ok = ~np.isnan(l) & (l > -np.inf)
+    if not ok.any():
+        return -1, 0.0, 1.0, {-1}
+    idx = np.nonzero(ok)[0]
+    rank = idx[np.lexsort((idx, -l[idx]))]
+    m = l[rank[0]]
+    if not T > 0:
+        return int(rank[0]), 1.0, 1.0, {int(rank[0])}
+    with np.errstate(invalid="ignore", over="ignore", under="ignore"):
+        w = np.where(l[rank] == m, 1.0, np.exp((l[rank] - m) / np.float64(np.float32(T))))
+    K = rank.size
+    if 1 <= k < V:
+        K = min(K, k)
+    near = 1.0
+    if p <= 0:
+        K = 1
+    elif p < 1:
+        c = np.cumsum(w[:K])
+        t = np.float64(np.float32(p)) * c[-1]
+        near = min(near, np.abs(np.delete(c, -1) - t).min() / c[-1]) if K > 1 else near
+        K = int(np.searchsorted(c, t, side="left")) + 1
+    K = min(K, rank.size)
+    if mp > 0:
+        K = min(K, int((w >= min(np.float64(np.float32(mp)), 1.0)).sum()))
+    kept = np.zeros(V)
+    kept[rank[:K]] = w[:K]
+    cdf = np.cumsum(kept)
+    u = np.float32(u)
+    u = min(max(float(u), 0.0), 1 - 2.0**-24) if u == u else 0.0
+    t = u * cdf[-1]
+    i = int(np.searchsorted(cdf, t, side="right"))
+    i = min(i, int(np.nonzero(kept)[0][-1]))
+    d = np.abs(cdf - t) / cdf[-1]
+    if u > 0:
+        near = min(near, d[kept > 0].min())
+    return i, kept[i] / cdf[-1], near, {i}
+
+
+def check(ops, logits, u, T=None, k=None, p=None, mp=None, cap=0.0, view=None):
+    """Runs the rows of `logits` (numpy f32) and compares each with the reference."""
+    R = logits.shape[0]
+    dev = (lambda a, t: None if a is None else torch.tensor(np.broadcast_to(np.asarray(a), (R,)).copy(), dtype=t, device="cuda"))
+    x = torch.from_numpy(np.ascontiguousarray(logits)).cuda() if view is None else view
+    ids, probs = ops.sample(x, dev(u, torch.float32), dev(T, torch.float32), dev(k, torch.int32), dev(p, torch.float32),
+                            dev(mp, torch.float32), cap=cap)
+    ids, probs = ids.cpu().numpy(), probs.cpu().numpy()
+    get = lambda a, r, d: d if a is None else np.broadcast_to(np.asarray(a), (R,))[r]  # noqa: E731
+    for r in range(R):
+        want, prob, near, _ = reference(logits[r], get(u, r, 0.0), get(T, r, 1.0), int(get(k, r, 0)), float(get(p, r, 1.0)),
+                                        float(get(mp, r, 0.0)))
+        if near < 1e-9:
+            continue
+        assert ids[r] == want, (r, ids[r], want, near)
+        assert abs(probs[r] - prob) <= 2.0**-23 * prob, (r, probs[r], prob)
+    return ids, probs
+
+
+def rows(R, V, seed, scale=2.5):
+    rng = np.random.default_rng(seed)
+    return (scale * rng.standard_normal((R, V))).astype(np.float32), rng.random(R).astype(np.float32)
+
+
+@pytest.mark.parametrize("V", [1, 2, 5, 31, 33, 127, 1000, 4099, 16385, 32003, 131073])
+def test_vocab_sizes(ops, V):
+    l, u = rows(9, V, V)
+    check(ops, l, u)
+    check(ops, l, u, T=0.7, k=np.arange(9) * 7)
+    check(ops, l, u, T=1.3, p=np.linspace(0.05, 0.99, 9), mp=0.01)
+
+
+@pytest.mark.parametrize("V", [262144, 300001, 786432])
+def test_large_vocabularies(ops, V):
+    l, u = rows(5, V, V, scale=3.0)
+    check(ops, l, u)
+    check(ops, l, u, T=0.8, k=[1, 64, 1000, 5000, V - 1], p=0.95)
+    check(ops, l, u, p=[0.1, 0.5, 0.9, 0.99, 0.9999])
+    check(ops, l, u, mp=[0.5, 0.1, 0.01, 0.001, 1e-6])
+
+
+@pytest.mark.parametrize("rows_", [1, 3, 148, 257])
+def test_row_counts(ops, rows_):
+    l, u = rows(rows_, 3001, rows_)
+    check(ops, l, u, T=np.linspace(0.3, 2.0, rows_), k=np.arange(rows_) % 90, p=0.9)
+
+
+def test_every_setting_at_its_edges(ops):
+    l, _ = rows(40, 2000, 4)
+    u = np.linspace(0, 1, 40).astype(np.float32)
+    check(ops, l, u, T=np.resize([0.0, -1.0, np.nan, 1e-30, 1e-3, 1e30, np.inf, 1.0], 40))
+    check(ops, l, u, k=np.resize([-5, 0, 1, 2, 1023, 1024, 1025, 1999, 2000, 2**31 - 1], 40))
+    check(ops, l, u, p=np.resize([-1.0, 0.0, 1e-7, 0.5, 0.999999, 1.0, 2.0, np.nan], 40).astype(np.float32))
+    check(ops, l, u, mp=np.resize([-1.0, 0.0, 1e-7, 0.3, 1.0, 5.0, np.nan], 40).astype(np.float32))
+    ids, _ = check(ops, l, np.resize([0.0, 1 - 2.0**-24, 1.0, 3.0, -1.0, np.nan], 40).astype(np.float32))
+    assert (ids >= 0).all()
+
+
+def test_masked_and_non_finite_logits(ops):
+    l, u = rows(8, 5000, 5)
+    l[0, :] = -np.inf
+    l[1, :] = np.nan
+    l[2, :] = -np.inf
+    l[2, 4321] = -3.4e38
+    l[3, ::2] = np.nan
+    l[4, 7] = l[4, 4000] = np.inf
+    l[5, :2500] = -np.inf
+    l[6, :] = np.finfo(np.float32).min
+    l[7, ::3] = np.finfo(np.float32).min
+    for kw in ({}, {"k": 50}, {"p": 0.8}, {"k": 2000, "p": 0.7, "mp": 0.05}):
+        ids, probs = check(ops, l, u, **kw)
+        assert ids[0] == -1 and ids[1] == -1 and probs[0] == 0 and ids[2] == 4321 and ids[4] in (7, 4000)
+
+
+@pytest.mark.parametrize("kw", [{}, {"k": 700}, {"k": 3}, {"p": 0.5}, {"p": 0.25, "k": 1000}, {"mp": 1.0}])
+def test_equal_logits(ops, kw):
+    """Ties go to the lowest index; the weights are whole numbers here, so every border is exact."""
+    R, V = 16, 8192
+    l = np.zeros((R, V), np.float32)
+    l[1::2, ::2] = -0.0  # -0 and +0 are equal
+    l[2, 100:] = -5.0
+    u = ((np.arange(R) + 0.37) / R).astype(np.float32)
+    check(ops, l, u, **kw)
+    few = np.random.default_rng(3).integers(0, 3, (R, V)).astype(np.float32)
+    check(ops, few, u, **kw)
+
+
+@pytest.mark.parametrize("order", ["falling", "rising", "blocks", "narrow", "wide"])
+def test_rows_in_hard_orders(ops, order):
+    """Rows whose large logits lie together, or whose values are nearly equal or far apart."""
+    V = 70001
+    l, u = rows(6, V, 11)
+    l = np.sort(l, axis=1)
+    if order == "falling":
+        l = l[:, ::-1].copy()
+    elif order == "blocks":
+        l = np.roll(l, V // 3, axis=1)
+    elif order == "narrow":
+        l = np.random.default_rng(1).permuted(l, axis=1) * np.float32(1e-4) + np.float32(20.0)
+    elif order == "wide":
+        l = np.random.default_rng(2).permuted(l, axis=1) * np.float32(1e4)
+    for kw in ({}, {"k": 64}, {"k": 1000}, {"k": 30000}, {"p": 0.3}, {"p": 0.95}, {"k": 40000, "p": 0.9}, {"mp": 0.2}):
+        check(ops, l, u, **kw)
+
+
+def test_strided_and_unaligned_rows(ops):
+    l, u = rows(7, 1003, 6)
+    big = torch.zeros((7, 2048), device="cuda")
+    for off in (0, 1, 2, 3, 4):
+        view = big[:, off:off + 1003]
+        view.copy_(torch.from_numpy(l))
+        check(ops, l, u, k=40, p=0.9, view=view)
+        check(ops, l, u, view=view)
+
+
+def test_cap_is_softcap_first(rt, ctx, ops):
+    """The same bits as g4_softcap in place and then no cap."""
+    l, u = rows(12, 9001, 8, scale=20.0)
+    x = torch.from_numpy(l).cuda()
+    U = torch.from_numpy(u).cuda()
+    k = torch.full((12,), 500, dtype=torch.int32, device="cuda")
+    got = ops.sample(x, U, top_k=k, cap=30.0)
+    full = ops.sample(x, U, cap=30.0)
+    rt.call("g4_softcap", ctx.handle, C.c_void_p(x.data_ptr()), x.numel(), C.c_float(30.0))
+    for a, b in ((got, ops.sample(x, U, top_k=k)), (full, ops.sample(x, U))):
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+def test_distribution_of_many_draws(ops):
+    """100,000 uniform numbers of an even grid on one row: each token's share is its probability to
+    within the grid's step (inverse of a cumulative sum)."""
+    l = np.array([[1.0, -2.0, 0.5, 3.0, 2.5, -1.0, 0.0]], np.float32)
+    n = 100000
+    u = ((np.arange(n) + 0.5) / n).astype(np.float32)
+    x = torch.from_numpy(l).cuda().expand(n, 7)
+    ids, _ = ops.sample(x.contiguous(), torch.from_numpy(u).cuda())
+    share = np.bincount(ids.cpu().numpy(), minlength=7) / n
+    w = np.exp(l[0].astype(np.float64))
+    assert np.abs(share - w / w.sum()).max() <= 2.0 / n
+
+
+def test_captured_call_replays_with_other_settings(rt):
+    """One captured call on a stream of its own reads the logits and settings of each replay."""
+    ctx = rt.Context(0)
+    ops = rt.GPUOps(ctx)
+    V, R = 20011, 5
+    side = torch.cuda.Stream()
+    x = torch.empty((R, V), device="cuda")
+    u, T, p = (torch.ones(R, device="cuda") for _ in range(3))
+    k = torch.zeros(R, dtype=torch.int32, device="cuda")
+    torch.cuda.synchronize()
+    ctx.set_stream(side)
+    with torch.cuda.stream(side):
+        x.zero_()
+        ops.sample(x, u, T, k, p)
+        side.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            ids, probs = ops.sample(x, u, T, k, p)
+        for seed in range(4):
+            l, un = rows(R, V, 100 + seed)
+            kk, pp = [0, 1, 50, 3000][seed], [1.0, 0.9, 0.5, 0.8][seed]
+            x.copy_(torch.from_numpy(l))
+            u.copy_(torch.from_numpy(un))
+            T.fill_(0.9), k.fill_(kk), p.fill_(pp)
+            g.replay()
+            side.synchronize()
+            for r in range(R):
+                want, prob, near, _ = reference(l[r], un[r], 0.9, kk, pp)
+                if near > 1e-9:
+                    assert int(ids[r]) == want
+
+
+def test_the_same_call_twice_gives_the_same_bits(ops):
+    l, u = rows(64, 100003, 9, scale=0.5)
+    x, U = torch.from_numpy(l).cuda(), torch.from_numpy(u).cuda()
+    p = torch.full((64,), 0.9, device="cuda")
+    a = ops.sample(x, U, top_p=p)
+    for _ in range(3):
+        b = ops.sample(x, U, top_p=p)
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+def test_refusals(rt, ops):
+    x = torch.zeros((2, 10), device="cuda")
+    u = torch.zeros(2, device="cuda")
+    for bad in (lambda: ops.sample(x.double(), u), lambda: ops.sample(x.cpu(), u), lambda: ops.sample(x, u[:1]),
+                lambda: ops.sample(x, u.double()), lambda: ops.sample(x.t(), torch.zeros(10, device="cuda")),
+                lambda: ops.sample(x, u, top_k=u), lambda: ops.sample(x, u, temperature=u.cpu()),
+                lambda: ops.sample(torch.zeros((2, 786433), device="cuda"), u)):
+        with pytest.raises(rt.G4Error):
+            bad()
+    ids, _ = ops.sample(x[:0], u[:0])
+    assert ids.numel() == 0
