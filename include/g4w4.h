@@ -407,7 +407,8 @@ typedef struct {
  * is base + its depth).  q, out: bf16 [rows, heads, hd], rows a multiple of nodes; logit scale
  * 1.0; heads 1..8, hd in {64,128,256,512}, q and out 16-byte aligned.  What masked cache rows
  * hold, NaN and infinity included, does not reach a row that does not see them; a row that sees
- * a value row (V) that is not finite is NaN throughout.  A sequence whose drafted rows would
+ * a value (V) that is not finite is NaN throughout (at hd 512: in the value's half of the
+ * columns).  A sequence whose drafted rows would
  * not fit its seq_stride (or a ring cache's capacity) is left out and raises
  * G4_DEVERR_BAD_INDEX.  Long key ranges are split over CTAs with partial results in the context
  * workspace (as g4_attention_rows).  G4_ROWS_HISTORY_READY as for g4_attention_rows. */
