@@ -479,7 +479,7 @@ g4_status make_kv_maps(g4_kv* kv) {
                                             CU_TENSOR_MAP_SWIZZLE_128B);
         if (st) return st;
     }
-    return G4_OK;
+    return make_tree_maps(kv);
 }
 
 template <int HD>

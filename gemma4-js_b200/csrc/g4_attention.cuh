@@ -21,10 +21,15 @@ struct g4_kv {
     uint16_t* v = nullptr;
     CUtensorMap kmap, vmap;     // 128B-swizzled boxes of 64 columns x (16384/hd) rows
     CUtensorMap kmap_narrow, vmap_narrow;  // the same with boxes of (8192/hd) rows
+    // Drafted-tree attention: [64 columns][rows][hd / 64] with boxes that fill a whole granule of
+    // its ring in one copy (g4_tree_attention.cu); a ring cache's boxes have at most `mirror` rows.
+    CUtensorMap tree_kmap, tree_vmap;
+    int tree_krows = 0, tree_vrows = 0;  // rows of their boxes
 };
 
 namespace g4 {
 g4_status make_kv_maps(g4_kv* kv);
+g4_status make_tree_maps(g4_kv* kv);  // part of make_kv_maps
 // A ring cache serves sliding attention with span + window - 1 <= ring only.
 g4_status check_ring(const char* name, const g4_kv* kv, int sliding, int window, int span);
 g4_status launch_attention(g4_ctx* ctx, const g4_kv* kv, int kv_row0, const uint16_t* q, int rows,

@@ -57,6 +57,10 @@ g4_status encode_tensor_map_2d(CUtensorMap* map, CUtensorMapDataType dtype, void
                                uint32_t box_inner, uint32_t box_outer,
                                CUtensorMapSwizzle swizzle);
 
+// The same of three dimensions; pitches of the two outer ones in bytes.
+g4_status encode_tensor_map_3d(CUtensorMap* map, CUtensorMapDataType dtype, void* base, const uint64_t (&dims)[3],
+                               const uint64_t (&pitch_bytes)[2], const uint32_t (&box)[3], CUtensorMapSwizzle swizzle);
+
 // Launches `kern` on the context stream with an optional thread-block cluster along x
 // and, when the context enables it, programmatic dependent launch: the kernel may start
 // while its predecessor drains, and waits (griddepcontrol.wait) before it touches any
@@ -218,6 +222,14 @@ __device__ __forceinline__ void tma_load_2d(void* smem_dst, const CUtensorMap* m
         "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
         " [%0], [%1, {%2, %3}], [%4];" ::"r"(smem_u32(smem_dst)),
         "l"(map), "r"(x), "r"(y), "r"(smem_u32(bar))
+        : "memory");
+}
+__device__ __forceinline__ void tma_load_3d(void* smem_dst, const CUtensorMap* map, uint64_t* bar,
+                                            int x, int y, int z) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_u32(smem_dst)),
+        "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
         : "memory");
 }
 __device__ __forceinline__ void bulk_load(void* smem_dst, const void* gsrc, uint32_t bytes,

@@ -97,6 +97,21 @@ g4_status encode_tensor_map_2d(CUtensorMap* map, CUtensorMapDataType dtype, void
     return G4_OK;
 }
 
+g4_status encode_tensor_map_3d(CUtensorMap* map, CUtensorMapDataType dtype, void* base, const uint64_t (&dims)[3],
+                               const uint64_t (&pitch_bytes)[2], const uint32_t (&box)[3], CUtensorMapSwizzle swizzle) {
+    auto fn = get_encode_fn();
+    if (!fn) return set_error(G4_ERR_CUDA, "cuTensorMapEncodeTiled entry point unavailable");
+    const cuuint64_t d[3] = {dims[0], dims[1], dims[2]}, st[2] = {pitch_bytes[0], pitch_bytes[1]};
+    const cuuint32_t b[3] = {box[0], box[1], box[2]}, estr[3] = {1, 1, 1};
+    const CUresult r = fn(map, dtype, 3, base, d, st, b, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS)
+        return set_error(G4_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d): dims %llu x %llu x %llu box %u x %u x %u", (int)r,
+                         (unsigned long long)dims[0], (unsigned long long)dims[1], (unsigned long long)dims[2], box[0],
+                         box[1], box[2]);
+    return G4_OK;
+}
+
 }  // namespace g4
 
 extern "C" {

@@ -11,6 +11,7 @@
 // reading the cache (at 148 SMs even one node's 8 rows keep the tensor pipe ahead of HBM), and
 // four CTAs of one sequence (64 nodes) by the products.
 #include <algorithm>
+#include <type_traits>
 
 #include "g4_attention.cuh"
 #include "g4_common.cuh"
@@ -24,7 +25,10 @@ using namespace g4dev;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kTile = 128;        // keys per tile = MMA N of the scores
 constexpr int kRowsPerCta = 128;  // MMA M
-constexpr int kSoftmaxThreads = 128;
+// Two threads per query row, each with half of a tile's keys and half of O's columns: two warps
+// per scheduler hide each other's latencies (one warp per scheduler: 4500 clocks per tile).
+constexpr int kSoftmaxWarps = 8;
+constexpr int kSoftmaxThreads = kSoftmaxWarps * 32;
 constexpr int kThreads = kSoftmaxThreads + 64;  // + TMA warp + MMA warp
 
 // Shared memory: Q [HD/64 boxes][128 rows][128 B], then a ring of equal slots that K and V
@@ -44,9 +48,8 @@ struct TreeCfg {
     static constexpr int VGRAN = HDV * 256 / SLOT;
     static constexpr int VKEYS = kTile / VGRAN;                // keys per V granule
     static constexpr int VBOX = VKEYS * 128;                   // bytes of a V box
-    static constexpr int BOXROWS = HD == 64 ? 128 : 16384 / HD;  // rows of a TMA box
     static constexpr int SLOTS = HD == 64 ? 8 : (229376 - QBYTES) / SLOT;
-    static constexpr int SMEM = QBYTES + SLOTS * SLOT + 2048;  // + alignment, barriers, parents
+    static constexpr int SMEM = QBYTES + SLOTS * SLOT + 3072;  // the rest: alignment (1008), TreeShared
     static_assert(SMEM <= 232448, "shared memory");
 };
 
@@ -59,6 +62,7 @@ struct TreeAttnParams {
     g4_tree tree;
     const int32_t* seq_pos;
     int seq_base, pos0, seq_stride, heads, sliding, window, ring, limit, nsplit, nseq, history_ready;
+    int krows, vrows;  // rows of the tensor maps' boxes (the whole granule, or a part in ring caches)
 };
 
 struct TreeShared {
@@ -67,6 +71,7 @@ struct TreeShared {
     uint32_t tmem;
     uint32_t poison[3][4];  // keys of a masked tile whose V row is not finite (three tiles in turn)
     int parents[G4_TREE_MAX_NODES];
+    float mx[2][2][kRowsPerCta];  // a row's maximum of each half (two tiles in turn); at the end its sums
 };
 
 __device__ __forceinline__ float ex2(float x) {  // 2^x to 2^-22, 0 for -inf
@@ -75,12 +80,35 @@ __device__ __forceinline__ float ex2(float x) {  // 2^x to 2^-22, 0 for -inf
     return y;
 }
 
-// MN-major operand in 128-byte swizzle: 64-element chunks `chunk` bytes apart, 8-row groups 1024 B apart.
-__device__ __forceinline__ uint64_t mn_desc(uint32_t saddr, uint32_t chunk) {
-    return (uint64_t)((saddr >> 4) & 0x3FFFu) | (uint64_t)(chunk >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 |
-           (uint64_t)1 << 46 | (uint64_t)2 << 61;
+// Shared-memory operand descriptors in 128-byte swizzle, 8-row groups 1024 B apart (g4_tcgen05.cuh:
+// sw128_desc), as two words: the high one is a constant, the low one moves by address / 16, so a
+// step costs the issuing thread one add (rebuilding the 64-bit descriptor per MMA: +25 clocks each).
+// `chunk`: for an MN-major operand, the distance of its 64-element chunks in bytes.
+constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_lo(uint32_t saddr, uint32_t chunk = 16) { return saddr >> 4 | (chunk >> 4) << 16; }
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
+        "mov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}" ::"r"(d),
+        "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(kDescHi));
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a_tmem, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\t"
+        "mov.b64 b, {%2, %5};\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}" ::"r"(d),
+        "r"(a_tmem), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(kDescHi));
+}
+__device__ __forceinline__ bool elect_one() {
+    uint32_t e;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(e));
+    return e != 0;
 }
 constexpr uint32_t kTransposeB = 1u << 16;
+// Weights (bf16 pairs) lie over the scores they come from, each half of a tile over its own half:
+// TMEM column of the 16-key step i.
+__device__ __forceinline__ int p_col(int i) { return (i >> 2) * 64 + (i & 3) * 8; }
 
 // Bits [lo, hi) of the word that covers columns 32 w .. 32 w + 31.
 __device__ __forceinline__ uint32_t range_word(int lo, int hi, int w) {
@@ -123,17 +151,29 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
     pdl_trigger();
     // With history_ready the positions and the cached rows below base are final already.
     if (!p.history_ready) pdl_wait();
+    // What the prologue reads goes out at once, before the first use of any of it.
+    constexpr int CH = HD / 8;  // 16-byte chunks per row
+    constexpr int PER = kRowsPerCta * CH / kSoftmaxThreads;
+    const int f0 = mtile * kRowsPerCta;
+    const size_t grow = (size_t)s * n * p.heads;  // the sequence's first row of q and out
+    const uint4* qg = reinterpret_cast<const uint4*>(p.q + (grow + f0) * HD);
+    int parent = -1;
+    auto prologue_loads = [&]() {
+        // Q into the swizzled operand layout.  Rows behind the sequence's count are products of no
+        // consequence; rows behind its nodes are zero.
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int u = i * kSoftmaxThreads + threadIdx.x, qr = u / CH, c = u % CH;
+            const bool in = f0 + qr < n * p.heads;
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                             smem_u32(qsm + (c >> 3) * 16384 + qr * 128 + (((c & 7) ^ (qr & 7)) << 4))),
+                         "l"(qg + (in ? u : 0)), "r"(in ? 16 : 0)
+                         : "memory");
+        }
+        if (threadIdx.x < n) parent = p.tree.parents[(size_t)s * p.tree.parent_stride + threadIdx.x];
+    };
     const TreeSeq ts = tree_seq(p, s);
-    // This split's tiles; tile t covers keys lo + (t0 + t) * 128 ...
-    const int t0 = (int)((long long)split * ts.ntiles / p.nsplit);
-    int nt = (int)((long long)(split + 1) * ts.ntiles / p.nsplit) - t0;
-    const int key0 = ts.lo + t0 * kTile;
-    if (ts.base < 0 || ts.base > p.limit) nt = 0;
-    if (!p.history_ready) {  // no used row among this CTA's
-        const int c = tree_count(p.tree, s, nullptr);
-        if (mtile * kRowsPerCta >= c * p.heads || !tree_seq_fits(p, ts, c)) nt = 0;
-    }
-
+    if (warp < kSoftmaxWarps && !p.history_ready) prologue_loads();
     if (threadIdx.x == 0) {
         for (int i = 0; i < C::SLOTS; ++i) {
             mbar_init(&sh.full[i], 1);
@@ -149,7 +189,16 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
         mbar_init(&sh.drained, 1);
         fence_mbar_init();
     }
-    if (warp == 5) tmem_alloc(&sh.tmem, 512);
+    if (warp == kSoftmaxWarps + 1) tmem_alloc(&sh.tmem, 512);
+    // This split's tiles; tile t covers keys lo + (t0 + t) * 128 ...
+    const int t0 = (int)((unsigned)split * (unsigned)ts.ntiles / (unsigned)p.nsplit);
+    int nt = (int)((unsigned)(split + 1) * (unsigned)ts.ntiles / (unsigned)p.nsplit) - t0;
+    const int key0 = ts.lo + t0 * kTile;
+    if (ts.base < 0 || ts.base > p.limit) nt = 0;
+    if (!p.history_ready) {  // no used row among this CTA's
+        const int c = tree_count(p.tree, s, nullptr);
+        if (mtile * kRowsPerCta >= c * p.heads || !tree_seq_fits(p, ts, c)) nt = 0;
+    }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -166,7 +215,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
     auto k_granule = [&](int t) { return t == 0 ? 0 : C::KGRAN + (t - 1) * G; };
     auto v_granule = [&](int t) { return C::KGRAN + t * G + (t + 1 < nt ? C::KGRAN : 0); };
 
-    if (warp == 4) {
+    if (warp == kSoftmaxWarps) {
         // ------------------------------------------------ TMA producer --
         if (lane == 0 && nt > 0) {
             prefetch_tensor_map(&kmap);
@@ -174,9 +223,19 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
             bool ok = true, waited = !p.history_ready;
             int g = 0;
             const int seq = p.seq_base + s;
-            auto load = [&](const CUtensorMap* map, int slot, uint32_t off, int x, int key) {
-                const int row = seq * p.seq_stride + (p.ring ? key % p.ring : key);
-                tma_load_2d(ring + slot * C::SLOT + off, map, &sh.full[slot], x, row);
+            // `boxes` 64-column boxes of `keys` keys, from column box `box`: one copy where the map's box
+            // covers them, else (a ring cache's rows are contiguous for `mirror` keys only) one per box and part.
+            auto load = [&](const CUtensorMap* map, int slot, int box, int boxes, int key, int keys, int part) {
+                uint8_t* to = ring + slot * C::SLOT;
+                const int row0 = seq * p.seq_stride;
+                if (part == keys) {
+                    tma_load_3d(to, map, &sh.full[slot], 0, row0 + (p.ring ? key % p.ring : key), box);
+                } else {
+                    for (int r = 0; r < keys; r += part)
+                        for (int b = 0; b < boxes; ++b)
+                            tma_load_3d(to + b * keys * 128 + r * 128, map, &sh.full[slot], 0, row0 + (key + r) % p.ring,
+                                        box + b);
+                }
             };
             auto claim = [&]() {
                 const int slot = g % C::SLOTS;
@@ -194,11 +253,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
                     for (int a = 0; a < C::KGRAN && ok; ++a, ++g) {
                         const int slot = claim();
                         if (!ok) break;
-#pragma unroll
-                        for (int b = 0; b < C::KBOXES; ++b)
-#pragma unroll
-                            for (int r = 0; r < kTile; r += C::BOXROWS)
-                                load(&kmap, slot, b * 16384 + r * 128, (a * C::KBOXES + b) * 64, k0 + r);
+                        load(&kmap, slot, a * C::KBOXES, C::KBOXES, k0, kTile, p.krows);
                     }
                 }
                 if (t >= 0) {
@@ -206,11 +261,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
                     for (int a = 0; a < C::VGRAN && ok; ++a, ++g) {
                         const int slot = claim();
                         if (!ok) break;
-#pragma unroll
-                        for (int b = 0; b < C::HDV / 64; ++b)
-#pragma unroll
-                            for (int r = 0; r < C::VKEYS; r += C::BOXROWS)
-                                load(&vmap, slot, b * C::VBOX + r * 128, vhalf * 256 + b * 64, k0 + a * C::VKEYS + r);
+                        load(&vmap, slot, vhalf * 4, C::HDV / 64, k0 + a * C::VKEYS, C::VKEYS, p.vrows);
                     }
                 }
             }
@@ -218,103 +269,119 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
             for (int i = g > C::SLOTS ? g - C::SLOTS : 0; i < g; ++i)
                 mbar_wait(&sh.full[i % C::SLOTS], (i / C::SLOTS) & 1, p.err, 702);
         }
-    } else if (warp == 5) {
+    } else if (warp == kSoftmaxWarps + 1) {
         // --------------------------------------------------- MMA issuer --
-        if (lane == 0 && nt > 0) {
+        // The warp stays together (its waits and addresses are uniform); one lane issues.
+        if (nt > 0) {
             constexpr uint32_t qk_idesc = mma_idesc_bf16(128, kTile);
             constexpr uint32_t pv_idesc = mma_idesc_bf16(128, C::HDV) | kTransposeB;
-            const uint32_t qa = smem_u32(qsm), ra = smem_u32(ring);
-            bool ok = mbar_wait(&sh.q_full, 0, p.err, 703);
+            const uint32_t qa = desc_lo(smem_u32(qsm)), ka = desc_lo(smem_u32(ring));
+            const uint32_t va = desc_lo(smem_u32(ring), C::VBOX);
+            bool ok = mbar_wait_warp(&sh.q_full, 0, p.err, 703);
+            int slot = 0;
+            uint32_t phase = 0;  // of the slot that comes next in ring order
+            auto next = [&]() {
+                if (++slot == C::SLOTS) slot = 0, phase ^= 1;
+            };
             auto scores = [&](int t) {
-                for (int a = 0; a < C::KGRAN && ok; ++a) {
-                    const int g = k_granule(t) + a, slot = g % C::SLOTS;
-                    ok = mbar_wait(&sh.full[slot], (g / C::SLOTS) & 1, p.err, 704);
+#pragma unroll
+                for (int a = 0; a < C::KGRAN; ++a) {
+                    ok = ok && mbar_wait_warp(&sh.full[slot], phase, p.err, 704);
                     if (!ok) return;
                     tc_fence_after();
+                    if (elect_one()) {
+                        const uint32_t b = ka + slot * (C::SLOT >> 4), d = tmem + (t & 1) * 128;
 #pragma unroll
-                    for (int i = 0; i < C::KBOXES * 4; ++i)
-                        tc_mma_ss(tmem + (t & 1) * 128, sw128_desc(qa + (a * C::KBOXES + i / 4) * 16384 + (i % 4) * 32),
-                                  sw128_desc(ra + slot * C::SLOT + (i / 4) * 16384 + (i % 4) * 32), qk_idesc,
-                                  (a | i) ? 1u : 0u);
-                    tc_commit(&sh.empty[slot]);
+                        for (int i = 0; i < C::KBOXES * 4; ++i)
+                            mma_ss(d, qa + (((a * C::KBOXES + i / 4) * 16384 + (i % 4) * 32) >> 4),
+                                   b + (((i / 4) * 16384 + (i % 4) * 32) >> 4), qk_idesc, (a | i) ? 1u : 0u);
+                        tc_commit(&sh.empty[slot]);
+                        if (a == C::KGRAN - 1) tc_commit(&sh.s_full[t & 1]);
+                    }
+                    __syncwarp();
+                    next();
                 }
-                tc_commit(&sh.s_full[t & 1]);
             };
             if (ok) scores(0);
             for (int t = 0; t < nt && ok; ++t) {
                 if (t + 1 < nt) scores(t + 1);
-                if (ok && masked_tile(t)) {  // hand V to the softmax threads (only this thread can follow the ring)
+                if (ok && masked_tile(t)) {  // hand V to the softmax threads (only this warp can follow the ring)
+                    int sl = slot;
+                    uint32_t ph = phase;
                     for (int a = 0; a < C::VGRAN && ok; ++a) {
-                        const int g = v_granule(t) + a;
-                        ok = mbar_wait(&sh.full[g % C::SLOTS], (g / C::SLOTS) & 1, p.err, 708);
+                        ok = mbar_wait_warp(&sh.full[sl], ph, p.err, 708);
+                        if (++sl == C::SLOTS) sl = 0, ph ^= 1;
                     }
-                    if (ok) mbar_arrive(&sh.v_full);
+                    if (ok && lane == 0) mbar_arrive(&sh.v_full);
+                    __syncwarp();
                 }
-                ok = ok && mbar_wait(&sh.p_ready[t & 1], (t >> 1) & 1, p.err, 705);
-                for (int a = 0; a < C::VGRAN && ok; ++a) {
-                    const int g = v_granule(t) + a, slot = g % C::SLOTS;
-                    ok = mbar_wait(&sh.full[slot], (g / C::SLOTS) & 1, p.err, 706);
+                ok = ok && mbar_wait_warp(&sh.p_ready[t & 1], (t >> 1) & 1, p.err, 705);
+#pragma unroll
+                for (int a = 0; a < C::VGRAN; ++a) {
+                    ok = ok && mbar_wait_warp(&sh.full[slot], phase, p.err, 706);
                     if (!ok) break;
                     tc_fence_after();
+                    if (elect_one()) {
+                        const uint32_t b = va + slot * (C::SLOT >> 4), w = tmem + (t & 1) * 128;
 #pragma unroll
-                    for (int i = 0; i < C::VKEYS / 16; ++i)
-                        tc_mma_ts(o_tmem, tmem + (t & 1) * 128 + (a * (C::VKEYS / 16) + i) * 8,
-                                  mn_desc(ra + slot * C::SLOT + i * 2048, C::VBOX), pv_idesc, (t | a | i) ? 1u : 0u);
-                    tc_commit(&sh.empty[slot]);
+                        for (int i = 0; i < C::VKEYS / 16; ++i)
+                            mma_ts(o_tmem, w + p_col(a * (C::VKEYS / 16) + i), b + i * (2048 >> 4), pv_idesc,
+                                   (a | i) || t > 0 ? 1u : 0u);
+                        tc_commit(&sh.empty[slot]);
+                        if (a == C::VGRAN - 1) tc_commit(&sh.o_done[t & 1]);
+                    }
+                    __syncwarp();
+                    next();
                 }
-                if (ok) tc_commit(&sh.o_done[t & 1]);
             }
             // Do not free the tensor memory while products may still be running (after a failed wait).
-            tc_commit(&sh.drained);
-            mbar_wait(&sh.drained, 0, p.err, 711);
+            if (elect_one()) tc_commit(&sh.drained);
+            __syncwarp();
+            mbar_wait_warp(&sh.drained, 0, p.err, 711);
         }
     } else {
-        // ------------------------------ softmax: thread = one query row --
-        if (p.history_ready) pdl_wait();
+        // ------------------ softmax: two threads (warps w, w + 4) per query row --
+        const int half = warp >> 2, r = (warp & 3) * 32 + lane;
+        const int f = f0 + r;
+        if (p.history_ready) {
+            pdl_wait();
+            prologue_loads();
+        }
         int count = tree_count(p.tree, s, p.err);
         if (!tree_seq_fits(p, ts, count)) {
             if (threadIdx.x == 0 && blockIdx.x == 0 && split == 0) raise_error(p.err, G4_DEVERR_BAD_INDEX);
             count = 0;
         }
-        if (threadIdx.x < n) sh.parents[threadIdx.x] = threadIdx.x < count ? tree_parent(p.tree, s, threadIdx.x, p.err) : -1;
+        if (threadIdx.x < n) {
+            const bool good = parent >= -1 && parent < (int)threadIdx.x;
+            if (!good && (int)threadIdx.x < count) raise_error(p.err, G4_DEVERR_BAD_INDEX);
+            sh.parents[threadIdx.x] = good ? parent : -1;
+        }
         if (threadIdx.x < 4) sh.poison[0][threadIdx.x] = 0u;
         const int rows = count * p.heads;              // of this sequence
-        const int f0 = mtile * kRowsPerCta, f = f0 + threadIdx.x;
-        const size_t grow = (size_t)s * n * p.heads;   // the sequence's first row of q and out
-        if (nt > 0) {
-            // Q into the swizzled operand layout; rows that are not used are zero.
-            constexpr int CH = HD / 8, PER = CH;       // 16-byte chunks per row = per thread
-            const uint4* qg = reinterpret_cast<const uint4*>(p.q + (grow + f0) * HD);
-            for (int i0 = 0; i0 < PER; i0 += 8) {
-                uint4 v[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int u = (i0 + i) * kSoftmaxThreads + threadIdx.x;
-                    v[i] = f0 + u / CH < rows ? qg[u] : make_uint4(0u, 0u, 0u, 0u);
-                }
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int u = (i0 + i) * kSoftmaxThreads + threadIdx.x, r = u / CH, c = u % CH;
-                    *reinterpret_cast<uint4*>(qsm + (c >> 3) * 16384 + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v[i];
-                }
-            }
-            fence_proxy_async_smem();
-            mbar_arrive(&sh.q_full);
-        }
-        asm volatile("bar.sync 1, 128;" ::: "memory");  // parents
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        fence_proxy_async_smem();
+        mbar_arrive(&sh.q_full);
+        asm volatile("bar.sync 1, 256;" ::: "memory");  // parents
         const bool live = f < rows;
         const bool warp_live = f - lane < rows;
         // The row's visible drafted rows (bit = node) and first visible cached key.
         unsigned long long seen = 0ull;
         int first = 0x7fffffff;
         if (live) {
-            const int node = f / p.heads;
             int up = 0;
-            for (int a = node; a >= 0; a = sh.parents[a], ++up)
+            for (int a = f / p.heads; a >= 0; a = sh.parents[a], ++up)
                 if (!p.sliding || up < p.window) seen |= 1ull << a;
             first = p.sliding ? ts.base + up - p.window : 0;  // up = depth + 1
         }
-        const uint32_t lane_off = (uint32_t)(warp * 32) << 16;
+        // Which of the keys k0 + 32 w .. + 31 the row sees.
+        auto visible = [&](int k0, int w) {
+            const int d = ts.base - k0, sft = 32 * w - d;  // node 0 is column d: the word's drafted bits start at node sft
+            const unsigned long long bits = sft >= 64 || sft <= -32 ? 0ull : sft >= 0 ? seen >> sft : seen << -sft;
+            return live ? range_word(first - k0, d, w) | (uint32_t)bits : 0u;
+        };
+        const uint32_t s_tmem = tmem + ((uint32_t)((warp & 3) * 32) << 16) + half * 64;
+        const uint32_t o_half = o_tmem + ((uint32_t)((warp & 3) * 32) << 16) + half * (C::HDV / 2);
         float m = -INFINITY, mu = 0.f, l = 0.f;
         // A warp whose wait gave up keeps to the barriers of the others and does nothing else.
         bool ok = true;
@@ -324,65 +391,33 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
             const bool masked = masked_tile(t);
             ok = ok && mbar_wait_warp(&sh.s_full[t & 1], (t >> 1) & 1, p.err, 707);
             tc_fence_after();
-            uint32_t vis[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
+            uint32_t vis[2] = {0xffffffffu, 0xffffffffu};
             if (masked) {
-                // What no row sees must not reach the product: 0 * NaN.  Thread = key: rows outside
-                // [lo, base + count) become 0; values that are not finite become 0 and are remembered.
-                const int key = k0 + threadIdx.x, vrow = threadIdx.x % C::VKEYS;
-                const int g = v_granule(t) + threadIdx.x / C::VKEYS;
-                uint32_t* poison = sh.poison[nmasked % 3];
-                if (threadIdx.x < 4) sh.poison[(nmasked + 1) % 3][threadIdx.x] = 0u;  // last read two masked tiles ago
-                ok = ok && mbar_wait_warp(&sh.v_full, nmasked & 1, p.err, 712);
-                ok = ok && mbar_wait_warp(&sh.full[g % C::SLOTS], (g / C::SLOTS) & 1, p.err, 713);  // of this phase now
-                ++nmasked;
-                if (ok) {
-                    uint8_t* vr = ring + (g % C::SLOTS) * C::SLOT + vrow * 128;
-                    const bool outside = key >= ts.base + count;
-                    bool bad = false;
-#pragma unroll 4
-                    for (int c = 0; c < C::HDV / 8; ++c) {
-                        uint4* at = reinterpret_cast<uint4*>(vr + (c >> 3) * C::VBOX + (((c & 7) ^ (vrow & 7)) << 4));
-                        uint4 w = *at;
-                        uint32_t* e = reinterpret_cast<uint32_t*>(&w);
-                        bool fix = outside;
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const bool b0 = (e[i] & 0x7f80u) == 0x7f80u, b1 = (e[i] & 0x7f800000u) == 0x7f800000u;
-                            if (outside) e[i] = 0u;
-                            else e[i] &= (b0 ? 0xffff0000u : 0xffffffffu) & (b1 ? 0x0000ffffu : 0xffffffffu);
-                            bad = bad || b0 || b1;
-                            fix = fix || b0 || b1;
-                        }
-                        if (fix) *at = w;
-                    }
-                    if (bad && !outside) atomicOr(&poison[threadIdx.x >> 5], 1u << lane);
-                    fence_proxy_async_smem();
-                }
-                asm volatile("bar.sync 1, 128;" ::: "memory");
-                const int d = ts.base - k0;  // column of node 0
-#pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    const int sft = 32 * w - d;  // drafted bits start at node sft
-                    const unsigned long long bits = sft >= 64 || sft <= -32 ? 0ull : sft >= 0 ? seen >> sft : seen << -sft;
-                    vis[w] = live ? range_word(first - k0, d, w) | (uint32_t)bits : 0u;
-                    if (vis[w] & poison[w]) l = __int_as_float(0x7fffffff);  // sees a V row that is not finite
-                }
+                vis[0] = visible(k0, 2 * half);
+                vis[1] = visible(k0, 2 * half + 1);
             }
+            float tm = -INFINITY;
             if (warp_live && ok) {
-                float x[kTile];
+#pragma unroll 1
+                for (int c = 0; c < 2; ++c) {
+                    uint32_t x[32];
+                    tmem_ld_32x32b_x32(s_tmem + (t & 1) * 128 + c * 32, x);
+                    tmem_ld_wait(x);
+                    if (masked) {
+                        const uint32_t v = c ? vis[1] : vis[0];
 #pragma unroll
-                for (int c = 0; c < 4; ++c)
-                    tmem_ld_32x32b_x32(tmem + lane_off + (t & 1) * 128 + c * 32, *reinterpret_cast<uint32_t(*)[32]>(x + c * 32));
+                        for (int i = 0; i < 32; ++i) x[i] = v >> i & 1u ? x[i] : 0xff800000u;
+                    }
+                    float m4[4] = {tm, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int c = 0; c < 4; ++c) tmem_ld_wait(*reinterpret_cast<uint32_t(*)[32]>(x + c * 32));
-                if (masked) {
-#pragma unroll
-                    for (int c = 0; c < kTile; ++c) x[c] = (vis[c >> 5] >> (c & 31)) & 1u ? x[c] : -INFINITY;
+                    for (int i = 0; i < 32; ++i) m4[i & 3] = fmaxf(m4[i & 3], __uint_as_float(x[i]));
+                    tm = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
                 }
-                float mx[4] = {x[0], x[1], x[2], x[3]};
-#pragma unroll
-                for (int c = 4; c < kTile; ++c) mx[c & 3] = fmaxf(mx[c & 3], x[c]);
-                const float tm = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                sh.mx[t & 1][half][r] = tm;
+            }
+            asm volatile("bar.sync %0, 64;" ::"r"(2 + (warp & 3)) : "memory");
+            if (warp_live && ok) {
+                tm = fmaxf(tm, sh.mx[t & 1][half ^ 1][r]);
                 // The weights are taken against a maximum that may be stale by up to 2^8 (P and the
                 // sums have the range for it), so O is rescaled only when it is exceeded.
                 const bool grow_m = tm > m && !((tm - m) * kLog2e <= 8.f);
@@ -397,132 +432,205 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
                     ok = mbar_wait_warp(&sh.o_done[(t - 1) & 1], ((t - 1) >> 1) & 1, p.err, 709);
                     tc_fence_after();
 #pragma unroll 1
-                    for (int c = 0; c < C::HDV; c += 32) {
+                    for (int c = 0; c < C::HDV / 2; c += 32) {
                         uint32_t o[32];
-                        tmem_ld_32x32b_x32(o_tmem + lane_off + c, o);
+                        tmem_ld_32x32b_x32(o_half + c, o);
                         tmem_ld_wait(o);
 #pragma unroll
                         for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * factor);
-                        tmem_st_32x32b_x32(o_tmem + lane_off + c, o);
+                        tmem_st_32x32b_x32(o_half + c, o);
                     }
                 }
                 // P in bf16 (the product's operand type; at most 1 part in 256 per weight) over the
                 // scores just read; l sums the rounded weights, so they are weights of sum 1.
-                float l0 = 0.f, l1 = 0.f;
+#pragma unroll 1
+                for (int c = 0; c < 2; ++c) {
+                    uint32_t x[32], w[16];
+                    tmem_ld_32x32b_x32(s_tmem + (t & 1) * 128 + c * 32, x);
+                    tmem_ld_wait(x);
+                    if (masked) {
+                        const uint32_t v = c ? vis[1] : vis[0];
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    uint32_t w[32];
+                        for (int i = 0; i < 32; ++i) x[i] = v >> i & 1u ? x[i] : 0xff800000u;
+                    }
+                    float l0 = 0.f, l1 = 0.f;
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        const float a = ex2(fmaf(x[h * 64 + 2 * i], kLog2e, -mu));
-                        const float b = ex2(fmaf(x[h * 64 + 2 * i + 1], kLog2e, -mu));
+                    for (int i = 0; i < 16; ++i) {
+                        const float a = ex2(fmaf(__uint_as_float(x[2 * i]), kLog2e, -mu));
+                        const float b = ex2(fmaf(__uint_as_float(x[2 * i + 1]), kLog2e, -mu));
                         asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[i]) : "f"(b), "f"(a));
                         l0 += __uint_as_float(w[i] << 16);
                         l1 += __uint_as_float(w[i] & 0xffff0000u);
                     }
-                    tmem_st_32x32b_x32(tmem + lane_off + (t & 1) * 128 + h * 32, w);
+                    tmem_st_32x32b_x16(s_tmem + (t & 1) * 128 + c * 16, w);
+                    l += l0 + l1;
                 }
-                l += l0 + l1;
                 tmem_st_wait();
+            }
+            if (masked) {
+                // What no row sees must not reach the product: 0 * NaN.  Thread = key and half of the
+                // columns: rows behind base + count become 0; values that are not finite become 0 and
+                // are remembered.
+                const int key = threadIdx.x & 127, vrow = key % C::VKEYS, g = v_granule(t) + key / C::VKEYS;
+                uint32_t* poison = sh.poison[nmasked % 3];
+                if (threadIdx.x < 4) sh.poison[(nmasked + 1) % 3][threadIdx.x] = 0u;  // last read two masked tiles ago
+                ok = ok && mbar_wait_warp(&sh.v_full, nmasked & 1, p.err, 712);
+                ok = ok && mbar_wait_warp(&sh.full[g % C::SLOTS], (g / C::SLOTS) & 1, p.err, 713);  // of this phase now
+                ++nmasked;
+                if (ok) {
+                    uint8_t* vr = ring + (g % C::SLOTS) * C::SLOT + vrow * 128;
+                    const bool outside = k0 + key >= ts.base + count;
+                    bool bad = false;
+                    auto at = [&](int i) {
+                        const int c = half * (C::HDV / 16) + i;
+                        return reinterpret_cast<uint4*>(vr + (c >> 3) * C::VBOX + (((c & 7) ^ (vrow & 7)) << 4));
+                    };
+                    // an exponent of all ones carries into the bit above it
+                    auto odd = [](uint32_t e) { return ((e & 0x7f807f80u) + 0x00800080u) & 0x80008000u; };
+                    uint32_t any = 0u;
+#pragma unroll 8
+                    for (int i = 0; i < C::HDV / 16; ++i) {
+                        const uint4 w = *at(i);
+                        any |= odd(w.x) | odd(w.y) | odd(w.z) | odd(w.w);
+                    }
+                    if (outside || any) {
+#pragma unroll 1
+                        for (int i = 0; i < C::HDV / 16; ++i) {
+                            const uint4 w = *at(i);
+                            auto clean = [&](uint32_t e) {
+                                const uint32_t o = odd(e);
+                                return outside ? 0u : e & ((o & 0x8000u ? 0u : 0xffffu) | (o & 0x80000000u ? 0u : 0xffff0000u));
+                            };
+                            *at(i) = make_uint4(clean(w.x), clean(w.y), clean(w.z), clean(w.w));
+                        }
+                        bad = !outside;
+                    }
+                    if (bad) atomicOr(&poison[key >> 5], 1u << lane);
+                    fence_proxy_async_smem();
+                }
+                asm volatile("bar.sync 1, 256;" ::: "memory");
+#pragma unroll 1
+                for (int w = 0; w < 4; ++w)
+                    if (poison[w] & visible(k0, w)) l = __int_as_float(0x7fffffff);  // sees a V row that is not finite
             }
             tc_fence_before();
             mbar_arrive(&sh.p_ready[t & 1]);
         }
         // ---- O of the row ----
-        if (nt > 0 && ok) ok = mbar_wait_warp(&sh.o_done[(nt - 1) & 1], ((nt - 1) >> 1) & 1, p.err, 710);
+        if (nt > 0) {
+            // mx[nt & 1] was last read before the barrier of tile nt - 1
+            sh.mx[nt & 1][half][r] = l;
+            asm volatile("bar.sync %0, 64;" ::"r"(2 + (warp & 3)) : "memory");
+            l += sh.mx[nt & 1][half ^ 1][r];
+            ok = ok && mbar_wait_warp(&sh.o_done[(nt - 1) & 1], ((nt - 1) >> 1) & 1, p.err, 710);
+        }
         tc_fence_after();
-        if (warp_live && ok) {
-            const float inv = 1.f / l;
-            const size_t row = grow + f;
+        // Rows leave through shared memory (Q and the ring have been read for the last time): written
+        // by row, 16-byte chunks permuted within 128 B against bank conflicts, read back along the
+        // rows, so that global stores are whole lines.  (Stores from the row's own thread touch 32
+        // lines each: 5 to 10 thousand clocks per CTA.)
+        if (nt > 0 && warp_live) {
             const size_t nrows = (size_t)p.nseq * n * p.heads;
-            if (p.nsplit > 1 && live) p.part_ml[(split * C::NV + vhalf) * nrows + row] = make_float2(mu, nt > 0 ? l : 0.f);
-            if (nt > 0) {
+            const float inv = 1.f / l;
+            auto stage = [&](auto whole_c) {
+                constexpr bool whole = decltype(whole_c)::value;
+                constexpr int rowb = C::HDV * (whole ? 2 : 4), chunks = rowb / 16;  // of a staged row
+                uint8_t* const mine = smem + r * rowb;
+                if (ok) {
 #pragma unroll 1
-                for (int c = 0; c < C::HDV; c += 32) {
-                    uint32_t o[32];
-                    tmem_ld_32x32b_x32(o_tmem + lane_off + c, o);
-                    tmem_ld_wait(o);
-                    if (!live) continue;
-                    if (p.nsplit == 1) {
-                        uint4* to = reinterpret_cast<uint4*>(p.out + row * HD + vhalf * 256 + c);
+                    for (int c = 0; c < C::HDV / 2; c += 32) {
+                        uint32_t o[32];
+                        tmem_ld_32x32b_x32(o_half + c, o);
+                        tmem_ld_wait(o);
+                        const int col = half * (C::HDV / 2) + c;
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
+                        for (int i = 0; i < (whole ? 4 : 8); ++i) {
                             uint32_t w[4];
 #pragma unroll
-                            for (int k = 0; k < 4; ++k)
-                                asm("cvt.rn.bf16x2.f32 %0, %1, %2;"
-                                    : "=r"(w[k])
-                                    : "f"(__uint_as_float(o[8 * i + 2 * k + 1]) * inv), "f"(__uint_as_float(o[8 * i + 2 * k]) * inv));
-                            to[i] = make_uint4(w[0], w[1], w[2], w[3]);
+                            for (int k = 0; k < 4; ++k) {
+                                if (whole)
+                                    asm("cvt.rn.bf16x2.f32 %0, %1, %2;"
+                                        : "=r"(w[k])
+                                        : "f"(__uint_as_float(o[(8 * i + 2 * k + 1) & 31]) * inv),
+                                          "f"(__uint_as_float(o[(8 * i + 2 * k) & 31]) * inv));
+                                else
+                                    w[k] = o[4 * i + k];
+                            }
+                            const int ch = (whole ? col / 8 : col / 4) + i;
+                            *reinterpret_cast<uint4*>(mine + (((ch & ~7) | ((ch ^ r) & 7)) << 4)) =
+                                make_uint4(w[0], w[1], w[2], w[3]);
                         }
-                    } else {
-                        uint4* to = reinterpret_cast<uint4*>(p.part_o + (split * nrows + row) * HD + vhalf * 256 + c);
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) to[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                    }
+                    if (!whole && live && half == 0)
+                        p.part_ml[(split * C::NV + vhalf) * nrows + grow + f] = make_float2(mu, l);
+                }
+                asm volatile("bar.sync %0, 64;" ::"r"(2 + (warp & 3)) : "memory");
+                if (ok) {
+                    const int row0 = (warp & 3) * 32;  // the pair's 32 rows
+                    uint8_t* const to = (whole ? reinterpret_cast<uint8_t*>(p.out) : reinterpret_cast<uint8_t*>(p.part_o)) +
+                                        ((whole ? 0 : split * nrows) + grow + f0) * (HD * (whole ? 2 : 4)) + vhalf * rowb;
+#pragma unroll 8
+                    for (int u = half * 32 + lane; u < 32 * chunks; u += 64) {
+                        const int rr = row0 + u / chunks, ch = u % chunks;
+                        if (f0 + rr < rows)
+                            *reinterpret_cast<uint4*>(to + (size_t)rr * (HD * (whole ? 2 : 4)) + ch * 16) =
+                                *reinterpret_cast<const uint4*>(smem + rr * rowb + (((ch & ~7) | ((ch ^ rr) & 7)) << 4));
                     }
                 }
-            }
+            };
+            if (p.nsplit == 1) stage(std::true_type{});
+            else stage(std::false_type{});
+        } else if (nt == 0 && p.nsplit > 1 && live && half == 0) {
+            const size_t nrows = (size_t)p.nseq * n * p.heads;
+            p.part_ml[(split * C::NV + vhalf) * nrows + grow + f] = make_float2(0.f, 0.f);
         }
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 5) {
+    if (warp == kSoftmaxWarps + 1) {
         __syncwarp();
         tc_fence_after();
         tmem_dealloc(tmem, 512);
     }
 }
 
-// Joins the splits of a row: out = sum_i 2^(mu_i - mu) O_i / sum_i 2^(mu_i - mu) l_i, one warp per
-// row and HDV columns.  A split that saw none of the row's keys has l = 0 and is left out (its O
-// is not read).
-constexpr int kCombineWarps = 4;
+// Joins the splits of a row: out = sum_i 2^(mu_i - mu) O_i / sum_i 2^(mu_i - mu) l_i.  One CTA per
+// row and HDV columns, a thread per two columns.  The splits' (mu, l) are read at once, then every
+// split's columns independently: two round trips.  A split that saw none of the row's keys has
+// l = 0 and is left out (its O was not written).
+constexpr int kMaxSplits = 160;
 template <int HD>
-__global__ void __launch_bounds__(kCombineWarps * 32) tree_combine_kernel(const TreeAttnParams p) {
+__global__ void __launch_bounds__(TreeCfg<HD>::HDV / 2) tree_combine_kernel(const TreeAttnParams p) {
     using C = TreeCfg<HD>;
+    constexpr int T = C::HDV / 2;
+    __shared__ float2 ml[kMaxSplits];
     pdl_trigger();
-    pdl_wait();
-    const int lane = threadIdx.x & 31, vhalf = blockIdx.y;
+    const size_t row = blockIdx.x;
+    const int vhalf = blockIdx.y;
     const size_t nrows = (size_t)p.nseq * p.tree.nodes * p.heads;
-    const size_t row = (size_t)blockIdx.x * kCombineWarps + (threadIdx.x >> 5);
-    if (row >= nrows) return;
     const int s = (int)(row / (p.tree.nodes * p.heads)), node = (int)(row / p.heads) - s * p.tree.nodes;
+    pdl_wait();
+    for (int i = threadIdx.x; i < p.nsplit; i += T) ml[i] = p.part_ml[(i * C::NV + vhalf) * nrows + row];
     const int count = tree_count(p.tree, s, nullptr);
-    if (node >= count || !tree_seq_fits(p, tree_seq(p, s), count)) return;
-    const float2* ml = p.part_ml + vhalf * nrows + row;
+    const bool used = node < count && tree_seq_fits(p, tree_seq(p, s), count);
+    __syncthreads();
+    if (!used) return;
     float mu = -INFINITY;
-    for (int i = lane; i < p.nsplit; i += 32) {
-        const float2 v = ml[i * (C::NV * nrows)];
-        if (v.y != 0.f) mu = fmaxf(mu, v.x);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mu = fmaxf(mu, __shfl_xor_sync(0xffffffffu, mu, o));
-    constexpr int E = C::HDV / 64;
-    float acc[2 * E], l = 0.f;
-#pragma unroll
-    for (int e = 0; e < 2 * E; ++e) acc[e] = 0.f;
-#pragma unroll 4
+    for (int i = 0; i < p.nsplit; ++i) mu = ml[i].y != 0.f ? fmaxf(mu, ml[i].x) : mu;
+    const float2* o = reinterpret_cast<const float2*>(p.part_o + row * HD + vhalf * C::HDV) + threadIdx.x;
+    float l = 0.f, a0 = 0.f, a1 = 0.f;
+#pragma unroll 8
     for (int i = 0; i < p.nsplit; ++i) {
-        const float2 v = ml[i * (C::NV * nrows)];
-        const bool use = v.y != 0.f;
-        const float f = use ? ex2(v.x - mu) : 0.f;
-        l += f * v.y;
-        const float2* o = reinterpret_cast<const float2*>(p.part_o + (i * nrows + row) * HD + vhalf * C::HDV);
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const float2 w = use ? o[e * 32 + lane] : make_float2(0.f, 0.f);
-            acc[2 * e] += f * w.x;
-            acc[2 * e + 1] += f * w.y;
-        }
+        const bool use = ml[i].y != 0.f;
+        const float f = use ? ex2(ml[i].x - mu) : 0.f;
+        const float2 v = use ? __ldg(o + i * nrows * (HD / 2)) : make_float2(0.f, 0.f);
+        l += f * ml[i].y;
+        a0 += f * v.x;
+        a1 += f * v.y;
     }
-    const float inv = 1.f / l;
-    uint32_t* out = reinterpret_cast<uint32_t*>(p.out + row * HD + vhalf * C::HDV);
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-        uint32_t w;
-        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(acc[2 * e + 1] * inv), "f"(acc[2 * e] * inv));
-        out[e * 32 + lane] = w;
-    }
+    uint32_t w;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(a1 / l), "f"(a0 / l));
+    reinterpret_cast<uint32_t*>(p.out + row * HD + vhalf * C::HDV)[threadIdx.x] = w;
 }
 
 template <int HD>
@@ -532,8 +640,11 @@ g4_status launch_tree_attention(g4_ctx* ctx, const g4_kv* kv, TreeAttnParams p) 
     const int longest = (p.sliding && p.window < p.seq_stride ? p.window : p.seq_stride) + p.tree.nodes;
     const int ntiles = (longest + kTile - 1) / kTile;
     const long long ctas = (long long)mtiles * C::NV * p.nseq;
-    // Split the keys while that adds CTAs to SMs without one, at two tiles or more per split.
-    int nsplit = (int)std::max<long long>(1, std::min<long long>(ctx->num_sms / ctas, ntiles / 2));
+    // Split the keys while that adds CTAs to SMs without one, at three tiles or more per split: a
+    // split costs its CTA's start and drain (about three tiles' time) and the join.  One sequence
+    // of 8 nodes over 4096 keys: 15.0 us at two tiles, 15.3 at three, 19.1 at six; 64 sequences
+    // with a window of 512 (five tiles): 28.6 us in two splits, 19.9 whole.
+    int nsplit = (int)std::max<long long>(1, std::min<long long>({ctx->num_sms / ctas, ntiles / 3, kMaxSplits}));
     p.nsplit = nsplit;
     if (nsplit > 1) {
         const size_t nrows = (size_t)p.nseq * p.tree.nodes * p.heads;
@@ -548,17 +659,51 @@ g4_status launch_tree_attention(g4_ctx* ctx, const g4_kv* kv, TreeAttnParams p) 
         G4_CHECK_CUDA(cudaFuncSetAttribute(tree_attention_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
         attr_set.fetch_or(1ull << ctx->device);
     }
-    const CUtensorMap& km = HD == 64 ? kv->kmap_narrow : kv->kmap;
-    const CUtensorMap& vm = HD == 64 ? kv->vmap_narrow : kv->vmap;
+    p.krows = kv->tree_krows;
+    p.vrows = kv->tree_vrows;
     g4_status st = g4::launch(ctx, "tree_attention_kernel", tree_attention_kernel<HD>, dim3(mtiles * C::NV, p.nseq, nsplit),
-                              dim3(kThreads), C::SMEM, 1, km, vm, p);
+                              dim3(kThreads), C::SMEM, 1, kv->tree_kmap, kv->tree_vmap, p);
     if (st || nsplit == 1) return st;
     const size_t nrows = (size_t)p.nseq * p.tree.nodes * p.heads;
-    return g4::launch(ctx, "tree_combine_kernel", tree_combine_kernel<HD>,
-                      dim3((unsigned)((nrows + kCombineWarps - 1) / kCombineWarps), C::NV), dim3(kCombineWarps * 32), 0, 1, p);
+    // The join is set up while the attention runs, and waits for it (griddepcontrol).
+    const bool pdl = ctx->pdl;
+    ctx->pdl = true;
+    st = g4::launch(ctx, "tree_combine_kernel", tree_combine_kernel<HD>,
+                      dim3((unsigned)nrows, C::NV), dim3(C::HDV / 2), 0, 1, p);
+    ctx->pdl = pdl;
+    return st;
+}
+
+template <int HD>
+g4_status tree_maps(g4_kv* kv) {
+    using C = TreeCfg<HD>;
+    const int contiguous = kv->ring ? kv->mirror : kTile;
+    kv->tree_krows = std::min(kTile, contiguous);
+    kv->tree_vrows = std::min(C::VKEYS, contiguous);
+    const uint64_t dims[3] = {64, (uint64_t)kv->rows_total, HD / 64}, pitch[2] = {HD * 2, 128};
+    const uint32_t kbox[3] = {64, (uint32_t)kv->tree_krows, kv->tree_krows == kTile ? (uint32_t)C::KBOXES : 1u};
+    const uint32_t vbox[3] = {64, (uint32_t)kv->tree_vrows, kv->tree_vrows == C::VKEYS ? C::HDV / 64u : 1u};
+    g4_status st = g4::encode_tensor_map_3d(&kv->tree_kmap, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, kv->k, dims, pitch, kbox,
+                                            CU_TENSOR_MAP_SWIZZLE_128B);
+    if (st) return st;
+    return g4::encode_tensor_map_3d(&kv->tree_vmap, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, kv->v, dims, pitch, vbox,
+                                    CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 }  // namespace
+
+namespace g4 {
+
+g4_status make_tree_maps(g4_kv* kv) {
+    switch (kv->hd) {
+        case 64: return tree_maps<64>(kv);
+        case 128: return tree_maps<128>(kv);
+        case 256: return tree_maps<256>(kv);
+        default: return tree_maps<512>(kv);
+    }
+}
+
+}  // namespace g4
 
 extern "C" g4_status g4_attention_tree(g4_ctx* ctx, const void* q_bf16, const g4_kv* kv, int rows, int heads, int hd,
                                        const g4_rows* map, const g4_tree* tree, int seq_stride, int sliding, int window,
