@@ -61,10 +61,11 @@ __device__ __forceinline__ float key_logit(uint32_t k) {
 // A row's settings with what is off made explicit.
 enum Mode { kTopK, kAll, kMinP, kTopP, kGeneral };
 struct RowSettings {
-    double c;         // log2(e) / temperature
+    float t;          // temperature
     double p, mp;     // p >= 1: off; mp = 0: off
     int k;            // 0: off
     Mode mode;
+    __device__ __forceinline__ double scale() const { return 1.4426950408889634 / (double)t; }  // log2(e) / T
 };
 __device__ __forceinline__ RowSettings row_settings(const SampleParams& P, int r) {
     RowSettings s;
@@ -75,9 +76,9 @@ __device__ __forceinline__ RowSettings row_settings(const SampleParams& P, int r
     if (s.k < 1 || s.k >= P.vocab) s.k = 0;
     s.p = tp < 1.f ? (double)tp : 2.0;
     s.mp = mp > 0.f ? fmin((double)mp, 1.0) : 0.0;
-    s.c = 1.4426950408889634 / (double)t;
+    s.t = t;
     if (!(t > 0.f)) {  // the greedy pick
-        s.k = 1, s.c = 1.0, s.p = 2.0, s.mp = 0.0;
+        s.k = 1, s.t = 1.f, s.p = 2.0, s.mp = 0.0;
     } else if (s.p <= 0.0) {
         s.k = 1, s.p = 2.0;
     }
@@ -85,34 +86,37 @@ __device__ __forceinline__ RowSettings row_settings(const SampleParams& P, int r
     return s;
 }
 
-// 2^y for y <= 0, relative error below 3e-15 (0 below 2^-1021): y = k / 32 + f, |f| <= 1/64, a
-// table of 2^(j/32) and the Taylor polynomial of 2^f to the fifth power (the table-driven method
-// of P. T. P. Tang, 1989).  12 double-precision operations; `table` is shared memory.
-__device__ __forceinline__ double exp2_64(double y, const double* table) {
-    const double magic = 211106232532992.0;  // 1.5 * 2^47: one unit in the last place is 1/32
-    const double t = y + magic;
-    const int k = __double2loint(t);
-    const double f = y - (t - magic);
-    double q = 0.0013333558146428443;
-    q = fma(q, f, 0.009618129107628477);
-    q = fma(q, f, 0.05550410866482158);
-    q = fma(q, f, 0.24022650695910072);
-    q = fma(q, f, 0.6931471805599453);
-    q = fma(q, f, 1.0);
-    q *= table[k & 31];
-    return y < -1021.0 ? 0.0 : __hiloint2double(__double2hiint(q) + ((k >> 5) << 20), __double2loint(q));
+// 2^(d c) for d c <= 0 to 2e-14 (0 below 2^-1021): d c = n + f with |f| <= 1/2, and the polynomial
+// of degree 9 that interpolates 2^f in the Chebyshev nodes of [-1/2, 1/2].  13 operations of the
+// double-precision pipe, 64 a clock and SM.  A table of 2^(j/32) in shared memory saves five of
+// them and costs more in bank conflicts: 52 us against 21 for the summary of 64 rows of 262144.
+__constant__ double kExp2[10] = {1.0000000000000135,    0.69314718055995,      0.240226506956403,     0.05550410866444768,
+                                 0.009618129193942167,  0.0013333558230170627, 0.00015403433746224196, 1.5252657257186041e-05,
+                                 1.3259646250270451e-06, 1.020869083593037e-07};
+__device__ __forceinline__ double exp2_64(double d, double c) {
+    const double magic = 6755399441055744.0;  // 1.5 * 2^52: one unit in the last place is 1
+    const double t = fma(d, c, magic);
+    const double f = fma(d, c, magic - t);
+    const int n = __double2loint(t);
+    double q = kExp2[9];
+#pragma unroll
+    for (int i = 8; i >= 0; --i) q = fma(q, f, kExp2[i]);
+    // The bits of t are those of magic plus n as a 64-bit number (a NaN's are not near).
+    const bool in = __double2hiint(t) - 0x43380000 == n >> 31 && n >= -1021;
+    return in ? __hiloint2double(__double2hiint(q) + (n << 20), __double2loint(q)) : 0.0;
 }
-__device__ __forceinline__ void fill_table(double* table) {
-    if (threadIdx.x < 32) table[threadIdx.x] = exp2((double)threadIdx.x * (1.0 / 32.0));
-}
-// exp((v - m) / T); +inf logits (m = +inf) share the whole weight.
-__device__ __forceinline__ double weight(float v, float m, double c, const double* table) {
-    if (v == m) return 1.0;
-    if (m == INFINITY) return 0.0;
-    return exp2_64(((double)v - (double)m) * c, table);
+// exp((v - m) / T), 0 for logits that are never picked; +inf logits (m = +inf) share the whole
+// weight.  Free of branches: the chains of several logits run beside one another (behind branches
+// they ran one after the other, 350 clocks each: 48 us against 19 for 64 rows of 262144).
+__device__ __forceinline__ double weight(float v, float m, double c) {
+    const double w = exp2_64((double)v - (double)m, c);
+    return v == m ? 1.0 : w;
 }
 
-__device__ __forceinline__ float capped(float v, float cap) { return cap > 0.f ? tanhf(v / cap) * cap : v; }
+// g4_softcap's arithmetic, but a mask (-inf) stays one; out of line, because 16 to 32 copies of it
+// in code that seldom runs it cost more in instruction fetches than the calls.
+__device__ __noinline__ float softcap(float v, float cap) { return v > -INFINITY ? tanhf(v / cap) * cap : v; }
+__device__ __forceinline__ float capped(float v, float cap) { return cap > 0.f ? softcap(v, cap) : v; }
 
 // ---------------------------------------------------------------- summary --
 // A warp takes 512 consecutive logits at a time as four chunks of 128.  kVec: rows are 16-byte
@@ -121,11 +125,8 @@ __device__ __forceinline__ float capped(float v, float cap) { return cap > 0.f ?
 constexpr int kSumWarps = 8;
 template <bool kVec>
 __global__ void __launch_bounds__(kSumWarps * 32) sample_summary_kernel(const SampleParams P, int segments) {
-    __shared__ double table[32];
     pdl_trigger();
     pdl_wait();
-    fill_table(table);
-    __syncthreads();
     if (blockIdx.x == 0 && threadIdx.x == 0) P.queue[0] = 0;
     const int lane = threadIdx.x & 31;
     const int r = (int)(blockIdx.x / (unsigned)segments);
@@ -137,7 +138,7 @@ __global__ void __launch_bounds__(kSumWarps * 32) sample_summary_kernel(const Sa
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         if (kVec && index(i, 3) < P.vocab) {
-            const float4 f = __ldcs(reinterpret_cast<const float4*>(row + index(i, 0)));
+            const float4 f = __ldg(reinterpret_cast<const float4*>(row + index(i, 0)));
             v[i][0] = f.x, v[i][1] = f.y, v[i][2] = f.z, v[i][3] = f.w;
         } else {
 #pragma unroll
@@ -150,7 +151,7 @@ __global__ void __launch_bounds__(kSumWarps * 32) sample_summary_kernel(const Sa
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[i][e] = capped(v[i][e], P.cap);
+            for (int e = 0; e < 4; ++e) v[i][e] = softcap(v[i][e], P.cap);
     }
     const int gs = 1 << P.gshift;
     // Units that one warp reduction covers: a chunk (kVec) or 32 logits of it.
@@ -161,9 +162,13 @@ __global__ void __launch_bounds__(kSumWarps * 32) sample_summary_kernel(const Sa
     for (int i = 0; i < 4; ++i) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            uint32_t k = kVec ? max(max(logit_key(v[i][0]), logit_key(v[i][1])), max(logit_key(v[i][2]), logit_key(v[i][3])))
-                              : logit_key(v[i][u]);
-            for (int o = 1; o < lanes; o <<= 1) k = max(k, __shfl_xor_sync(0xffffffffu, k, o));
+            // fmaxf passes over NaN
+            uint32_t k = logit_key(kVec ? fmaxf(fmaxf(v[i][0], v[i][1]), fmaxf(v[i][2], v[i][3])) : v[i][u]);
+            if (lanes == 32) {
+                k = __reduce_max_sync(0xffffffffu, k);
+            } else {
+                for (int o = 1; o < lanes; o <<= 1) k = max(k, __shfl_xor_sync(0xffffffffu, k, o));
+            }
             key[i][u] = k;
         }
     }
@@ -191,6 +196,7 @@ __global__ void __launch_bounds__(kSumWarps * 32) sample_summary_kernel(const Sa
     }
     double sum[4][U];
     if (mass) {
+        const double c = st.scale();
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
 #pragma unroll
@@ -198,9 +204,7 @@ __global__ void __launch_bounds__(kSumWarps * 32) sample_summary_kernel(const Sa
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int u = kVec ? 0 : e;
-                const uint32_t k = key[i][u];
-                const float g = key_logit(k);
-                if (k != 0u && logit_key(v[i][e]) != 0u) sum[i][u] += weight(v[i][e], g, st.c, table);
+                sum[i][u] += weight(v[i][e], key_logit(key[i][u]), c);  // a group without any: against NaN, 0
             }
 #pragma unroll
             for (int u = 0; u < U; ++u)
@@ -275,9 +279,9 @@ __device__ __forceinline__ double block_sum(double v, BlockScratch& s, int& flip
     flip ^= 1;
     if ((threadIdx.x & 31) == 0) s.d[flip][threadIdx.x >> 5] = v;
     __syncthreads();
-    double t = 0.0;
+    double t = s.d[flip][threadIdx.x & (kWarps - 1)];
 #pragma unroll
-    for (int i = 0; i < kWarps; ++i) t += s.d[flip][i];
+    for (int o = kWarps / 2; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
     return t;
 }
 // Sum over the threads before this one; *total gets the whole.
@@ -292,32 +296,77 @@ __device__ __forceinline__ double block_prefix(double v, BlockScratch& s, int& f
     flip ^= 1;
     if (lane == 31) s.d[flip][w] = x;
     __syncthreads();
-    double before = 0.0, all = 0.0;
+    double y = lane < kWarps ? s.d[flip][lane] : 0.0;  // sums of the warps up to and with `lane`
 #pragma unroll
-    for (int i = 0; i < kWarps; ++i) {
-        if (i == w) before = all;
-        all += s.d[flip][i];
+    for (int o = 1; o < kWarps; o <<= 1) {
+        const double z = __shfl_up_sync(0xffffffffu, y, o);
+        if (lane >= o) y += z;
     }
-    *total = all;
+    *total = __shfl_sync(0xffffffffu, y, kWarps - 1);
+    double before = __shfl_sync(0xffffffffu, y, w > 0 ? w - 1 : 0);
+    if (w == 0) before = 0.0;
     double left = __shfl_up_sync(0xffffffffu, x, 1);
     if (lane == 0) left = 0.0;
     return before + left;
 }
 
-// Bitonic sort of n = a power of two 64-bit values in shared memory, largest first.
-__device__ __forceinline__ void block_sort_desc(unsigned long long* a, int n) {
-    for (int size = 2; size <= n; size <<= 1) {
+// Bitonic sort of n2 = a power of two up to kThreads * E 64-bit values in shared memory, largest
+// first.  Values stay in registers (value e * kThreads + t in thread t): partners less than 32 away
+// come by shuffle, more than the block away from the thread itself, the others through `a` and
+// `b` in turn, one barrier a step (18 of the 66 steps of 2048 values).
+template <int E>
+__device__ __forceinline__ void block_sort_desc(unsigned long long* a, unsigned long long* b, int n2) {
+    const int t = threadIdx.x;
+    unsigned long long v[E];
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = e * kThreads + t < n2 ? a[e * kThreads + t] : 0ull;
+    bool second = true;  // the buffer that may be written: a's values have been read after the next barrier
+    for (int size = 2; size <= n2; size <<= 1) {
         for (int step = size >> 1; step > 0; step >>= 1) {
-            __syncthreads();
-            for (int t = threadIdx.x; t < n / 2; t += kThreads) {
-                const int i = 2 * t - (t & (step - 1)), j = i + step;
-                const unsigned long long x = a[i], y = a[j];
-                const bool desc = (i & size) == 0;
-                if ((x < y) == desc) a[i] = y, a[j] = x;
+            if (step >= kThreads) {
+                const int de = step / kThreads;
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+#pragma unroll
+                    for (int f = e + 1; f < E; ++f) {
+                        if (f != (e ^ de)) continue;
+                        const bool desc = ((e * kThreads + t) & size) == 0;
+                        if ((v[e] < v[f]) == desc) {
+                            const unsigned long long x = v[e];
+                            v[e] = v[f], v[f] = x;
+                        }
+                    }
+                }
+                continue;
+            }
+            unsigned long long* const buf = second ? b : a;
+            if (step >= 32) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) buf[e * kThreads + t] = v[e];
+                __syncthreads();
+                second = !second;
+            }
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const int i = e * kThreads + t;
+                const unsigned long long o = step >= 32 ? buf[i ^ step] : __shfl_xor_sync(0xffffffffu, v[e], step);
+                const bool larger = ((i & size) == 0) == ((i & step) == 0);  // this one keeps the larger
+                v[e] = (o > v[e]) == larger ? o : v[e];
             }
         }
     }
     __syncthreads();
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+        if (e * kThreads + t < n2) a[e * kThreads + t] = v[e];
+    __syncthreads();
+}
+template <int E>
+__device__ __forceinline__ void block_sort_desc_any(unsigned long long* a, unsigned long long* b, int n2) {
+    if (n2 <= kThreads) block_sort_desc<1>(a, b, n2);
+    else if (n2 <= 2 * kThreads) block_sort_desc<2>(a, b, n2);
+    else block_sort_desc<E>(a, b, n2);
 }
 __device__ __forceinline__ int pow2_at_least(int n) { return n <= 2 ? 2 : 1 << (32 - __clz(n - 1)); }
 
@@ -327,22 +376,87 @@ __device__ __forceinline__ double row_uniform(const SampleParams& P, int r) {
 }
 
 // ----------------------------------------------------------------- finish --
+constexpr int kFew = 256;
 struct FinishShared {
-    double table[32];
-    unsigned long long cand[kCand];  // key << 32 | ~index; then index << 32 | position
+    unsigned long long cand[kCand];  // key << 32 | ~index; then ~index << 32 | position
+    unsigned long long cand2[kCand];
     double w[kCand];
     uint16_t glist[kMaxGroups];
     BlockScratch scratch;
     double zk;
-    int n, ng, kept;
+    int n, ng, kept, found, pick;
+    uint32_t hist[256], found_above, found_in;
+    int rank[kFew];
 };
+
+// The end of a row with at most kFew candidates: ranks by counting (several threads per candidate)
+// instead of sorts, whose 28 barriers for 128 candidates cost 6400 clocks.
+template <class Leave>
+__device__ __forceinline__ void finish_few(const SampleParams& P, FinishShared& S, const RowSettings& st, int r, int n,
+                                           float m, double c, double u, double total, int& flip, Leave leave) {
+    const int n2 = max(32, pow2_at_least(n)), parts = kThreads / n2, part = threadIdx.x / n2, i = threadIdx.x & (n2 - 1);
+    const int t = threadIdx.x;
+    if (i < n) {
+        const unsigned long long me = S.cand[i];
+        int above = 0;
+#pragma unroll 4
+        for (int j = part; j < n; j += parts) above += S.cand[j] > me;
+        if (above) atomicAdd(&S.rank[i], above);
+    }
+    __syncthreads();
+    unsigned long long* sorted = S.cand + kFew;
+    if (t < n) sorted[S.rank[t]] = S.cand[t];
+    __syncthreads();
+    const int limit = st.mode == kTopK ? min(st.k, n) : n;
+    const double w = t < limit ? weight(key_logit((uint32_t)(sorted[t] >> 32)), m, c) : 0.0;
+    if (t < n) S.w[t] = w;
+    if (t == 0) S.kept = limit;
+    double all;
+    const double run = block_prefix(w, S.scratch, flip, &all) + w;
+    if (st.mode != kTopP) total = all;
+    const double need = st.p * total;
+    if (st.mode == kTopP && all < need) {
+        leave();
+        return;
+    }
+    // kept: the shortest prefix of the filters.
+    if (t < limit && ((st.p < 1.0 && run >= need) || (t + 1 < limit && st.mp > 0.0 && S.w[t + 1] < st.mp)))
+        atomicMin(&S.kept, t + 1);
+    __syncthreads();
+    const int kept = S.kept;
+    if (t == kept - 1) S.zk = run;
+    // What lies before each kept one in index order.
+    double* before = S.w + kFew;  // [parts][n2]
+    if (i < kept) {
+        const uint32_t me = (uint32_t)sorted[i];  // ~index
+        double s0 = 0.0;
+#pragma unroll 4
+        for (int j = part; j < kept; j += parts) s0 += (uint32_t)sorted[j] > me ? S.w[j] : 0.0;
+        before[part * n2 + i] = s0;
+    }
+    __syncthreads();
+    const double target = u * S.zk;
+    int mine = -1;
+    if (t < kept && w > 0.0) {
+        double s0 = 0.0;
+        for (int q = 0; q < parts; ++q) s0 += before[q * n2 + t];
+        mine = (int)(0xffffffffu - (uint32_t)sorted[t]);
+        // the highest index with no more than the target before it
+        if (s0 <= target) atomicMax(&S.pick, mine);
+    }
+    __syncthreads();
+    if (mine >= 0 && mine == S.pick) {
+        P.ids[r] = mine;
+        if (P.probs) P.probs[r] = (float)(w / S.zk);
+    }
+}
 
 __global__ void __launch_bounds__(kThreads) sample_finish_kernel(const SampleParams P, int vec) {
     extern __shared__ __align__(16) uint8_t smem_raw[];
     FinishShared& S = *reinterpret_cast<FinishShared*>(smem_raw);
     pdl_trigger();
-    fill_table(S.table);
-    if (threadIdx.x == 0) S.n = S.ng = S.kept = 0;
+    if (threadIdx.x == 0) S.n = S.ng = S.kept = 0, S.pick = -1;
+    if (threadIdx.x < kFew) S.rank[threadIdx.x] = 0;
     pdl_wait();
     int flip = 0;
     const int r = blockIdx.x, G = P.groups, gs = 1 << P.gshift;
@@ -381,12 +495,13 @@ __global__ void __launch_bounds__(kThreads) sample_finish_kernel(const SamplePar
     }
     if (st.mode == kAll) {
         // Groups in index order, four consecutive ones per thread.
+        const double c = st.scale();
         const double* gm = P.gmass + (size_t)r * G;
         double x[KG], own = 0.0, total;
 #pragma unroll
         for (int i = 0; i < KG; ++i) {
             const int g = threadIdx.x * KG + i;
-            x[i] = g < G && gk[g] ? gm[g] * weight(key_logit(gk[g]), m, st.c, S.table) : 0.0;
+            x[i] = g < G && gk[g] ? gm[g] * weight(key_logit(gk[g]), m, c) : 0.0;
             own += x[i];
         }
         const double before = block_prefix(own, S.scratch, flip, &total);
@@ -399,22 +514,22 @@ __global__ void __launch_bounds__(kThreads) sample_finish_kernel(const SamplePar
         }
         __syncthreads();
         if (S.ng == (int)threadIdx.x + 1) {
-            double c = before;
+            double run = before;
             int g = 0;
 #pragma unroll
             for (int i = 0; i < KG; ++i) {
-                if (x[i] > 0.0 && c <= target) {
+                if (x[i] > 0.0 && run <= target) {
                     g = threadIdx.x * KG + i;
-                    S.w[0] = c;
+                    S.w[0] = run;
                 }
-                c += x[i];
+                run += x[i];
             }
             S.n = g;
         }
         __syncthreads();
         if (threadIdx.x < 32) {  // the pick inside the group
             const int lane = threadIdx.x;
-            double c = S.w[0];
+            double run = S.w[0];
             int pick = -1;
             double wp = 0.0;
             for (int o = 0; o < gs; o += 32) {
@@ -422,7 +537,7 @@ __global__ void __launch_bounds__(kThreads) sample_finish_kernel(const SamplePar
                 double w = 0.0;
                 if (o + lane < gs && i < P.vocab) {
                     const float v = capped(row[i], P.cap);
-                    if (logit_key(v)) w = weight(v, m, st.c, S.table);
+                    if (logit_key(v)) w = weight(v, m, c);
                 }
                 double s = w;
 #pragma unroll
@@ -430,7 +545,7 @@ __global__ void __launch_bounds__(kThreads) sample_finish_kernel(const SamplePar
                     const double y = __shfl_up_sync(0xffffffffu, s, d);
                     if (lane >= d) s += y;
                 }
-                const unsigned past = __ballot_sync(0xffffffffu, w > 0.0 && c + s > target);
+                const unsigned past = __ballot_sync(0xffffffffu, w > 0.0 && run + s > target);
                 const unsigned some = __ballot_sync(0xffffffffu, w > 0.0);
                 const int from = past ? __ffs(past) - 1 : some ? 31 - __clz(some) : 0;
                 if (some) {
@@ -438,7 +553,7 @@ __global__ void __launch_bounds__(kThreads) sample_finish_kernel(const SamplePar
                     wp = __shfl_sync(0xffffffffu, w, from);
                 }
                 if (past) break;
-                c += __shfl_sync(0xffffffffu, s, 31);
+                run += __shfl_sync(0xffffffffu, s, 31);
             }
             if (lane == 0) {
                 P.ids[r] = pick;
@@ -449,106 +564,169 @@ __global__ void __launch_bounds__(kThreads) sample_finish_kernel(const SamplePar
     }
 
     // Candidates: every logit with key >= bound, from the groups whose maximum reaches it.
+    const double c = st.scale();
     uint32_t bound;
     double total = 0.0;
     if (st.mode == kMinP) {
-        // the lowest key that weighs mp or more: w falls with the key
+        // The lowest key that weighs mp or more (w falls with the key): every thread tries one of 512
+        // keys of what is left.
         uint32_t lo = kLowestKey, hi = top;  // hi keeps
+        const double at = (double)m + (double)st.t * log(st.mp);  // where it is, but for roundings
+        if (m < 3.0e38f && at > -3.0e38) {
+            const uint32_t k = logit_key((float)at);
+            const uint32_t a = max(k, kLowestKey + 200u) - 200u, b = min(k + 200u, top);
+            if (a < b && weight(key_logit(b), m, c) >= st.mp && weight(key_logit(a), m, c) < st.mp) lo = a, hi = b;
+        }
         while (lo < hi) {
-            const uint32_t mid = lo + (hi - lo) / 2;
-            if (weight(key_logit(mid), m, st.c, S.table) >= st.mp) hi = mid;
-            else lo = mid + 1;
+            const uint32_t span = hi - lo;
+            auto cut = [&](int t) { return lo + (uint32_t)((unsigned long long)span * (unsigned)t / kThreads); };
+            const int below = __syncthreads_count(weight(key_logit(cut(threadIdx.x)), m, c) < st.mp);
+            const uint32_t nhi = below < kThreads ? cut(below) : hi;
+            lo = below > 0 ? cut(below - 1) + 1 : lo;
+            hi = nhi;
         }
         bound = hi;
     } else {
-        low = ~block_max(low, S.scratch, flip);  // the lowest group maximum
-        uint32_t lo = low, hi = top + 1;          // [lo, hi): what counts >= lo is enough, >= hi is not
+        // The highest bound that the group maxima reach often enough (top-k: k of them; top-p: maxima
+        // that weigh what is needed, in units of 2^-20), by a histogram of what is left in 256 parts.
+        low = ~block_max(low, S.scratch, flip);
+        uint32_t val[KG], need;
         if (st.mode == kTopK) {
-            int c = 0;
 #pragma unroll
-            for (int i = 0; i < KG; ++i) c += key[i] != 0u;
-            if (block_sum_int(c, S.scratch, flip) < st.k) {
-                lo = 1;
-            } else {
-                while (hi - lo > 1) {
-                    const uint32_t mid = lo + (hi - lo) / 2;
-                    c = 0;
-#pragma unroll
-                    for (int i = 0; i < KG; ++i) c += key[i] >= mid;
-                    c = block_sum_int(c, S.scratch, flip);
-                    if (c >= st.k) {
-                        lo = mid;
-                        if (c <= st.k + st.k / 8 + 4) break;  // few enough
-                    } else {
-                        hi = mid;
-                    }
-                }
-            }
+            for (int i = 0; i < KG; ++i) val[i] = 1;
+            need = (uint32_t)st.k;
         } else {
-            // Nucleus: the weights of the highest group maxima are a lower bound of what the logits
-            // above them weigh.
             const double* gm = P.gmass + (size_t)r * G;
             double own = 0.0;
-            float w[KG];
 #pragma unroll
             for (int i = 0; i < KG; ++i) {
                 const int g = i * kThreads + threadIdx.x;
-                const double x = key[i] ? weight(key_logit(key[i]), m, st.c, S.table) : 0.0;
-                w[i] = (float)x;
-                own += key[i] ? x * gm[g] : 0.0;
+                const double x = weight(key_logit(key[i]), m, c);
+                val[i] = (uint32_t)(x * 1048576.0);
+                own += g < G ? x * gm[g] : 0.0;
             }
             total = block_sum(own, S.scratch, flip);
-            const float need = (float)(st.p * total * 1.0001);
-            auto above = [&](uint32_t at) {
-                float s = 0.f;
-#pragma unroll
-                for (int i = 0; i < KG; ++i) s += key[i] >= at ? w[i] : 0.f;
-                return block_sum((double)s, S.scratch, flip);
-            };
-            if (above(low) < need) {
+            const double fixed = st.p * total * 1048576.0 + kMaxGroups;
+            if (fixed > 2147483648.0) {  // more than all maxima can weigh
                 leave();
                 return;
             }
-            while (hi - lo > 1) {
-                const uint32_t mid = lo + (hi - lo) / 2;
-                const double a = above(mid);
-                if (a >= need) {
-                    lo = mid;
-                    if (a <= need * 1.01) break;
-                } else {
-                    hi = mid;
+            need = (uint32_t)fixed;
+        }
+        uint32_t lo = low, hi = top + 1, above = 0;
+        bool enough = false;
+        if (st.mode == kTopK && st.k <= kThreads / 4) {
+            // Few: the maxima of each thread's four groups will do, one barrier per halving.
+            uint32_t mine = 0;
+#pragma unroll
+            for (int i = 0; i < KG; ++i) mine = max(mine, key[i]);
+            if (__syncthreads_count(mine >= low) >= st.k) {
+                enough = true;
+                while (hi - lo > 1) {
+                    const uint32_t mid = lo + (hi - lo) / 2;
+                    const int count = __syncthreads_count(mine >= mid);
+                    if (count >= st.k) lo = mid;
+                    else hi = mid;
+                    if (count >= st.k && count <= st.k + st.k / 8 + 4) break;
                 }
             }
         }
-        bound = lo;
+        for (bool done = enough; !done;) {
+            const uint32_t span = hi - lo;
+            const int shift = max(0, 24 - __clz(span - 1 | 1u));
+            if (threadIdx.x < 256) S.hist[threadIdx.x] = 0;
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < KG; ++i)
+                if (key[i] >= lo && key[i] < hi && key[i]) atomicAdd(&S.hist[(key[i] - lo) >> shift], val[i]);
+            __syncthreads();
+            if (threadIdx.x < 32) {  // lane l: parts 8 l .. 8 l + 7; sums from the top
+                uint32_t h[8], sum = 0;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) sum += h[i] = S.hist[threadIdx.x * 8 + i];
+                uint32_t from = sum;  // of this lane's parts and all above
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const uint32_t x = __shfl_down_sync(0xffffffffu, from, o);
+                    if (threadIdx.x + o < 32) from += x;
+                }
+                const unsigned ok = __ballot_sync(0xffffffffu, above + from >= need);
+                if (ok == 0u) {
+                    if (threadIdx.x == 0) S.found = -1;
+                } else if ((int)threadIdx.x == 31 - __clz(ok)) {
+                    uint32_t run = above + from - sum;
+                    int at = 7;
+#pragma unroll
+                    for (int i = 7; i >= 0; --i) {
+                        at = i;
+                        if (run + h[i] >= need) break;
+                        run += h[i];
+                    }
+                    S.found = threadIdx.x * 8 + at;
+                    S.found_above = run;
+                    S.found_in = h[at];
+                }
+            }
+            __syncthreads();
+            const int at = S.found;
+            if (at < 0) break;  // all of the maxima are not enough
+            enough = true;
+            const uint32_t part = lo + ((uint32_t)at << shift);
+            if (hi - part > 1u << shift) hi = part + (1u << shift);
+            lo = part;
+            above = S.found_above;
+            if (shift == 0 || above + S.found_in <= need + need / 8 + (st.mode == kTopK ? 4 : 0)) done = true;
+        }
+        if (!enough && st.mode == kTopP) {
+            leave();
+            return;
+        }
+        bound = enough ? lo : 1u;
     }
 #pragma unroll
     for (int i = 0; i < KG; ++i)
         if (key[i] >= bound) S.glist[atomicAdd(&S.ng, 1)] = (uint16_t)(i * kThreads + threadIdx.x);
     __syncthreads();
     const int ng = S.ng;
-    if (ng > kCand / 2 && P.vocab > 4 * kCand) {  // too many to rank here (a short row is tried whole)
+    // Too many to read here (a short row is tried whole): by one CTA 1024 groups take 60 us, by the
+    // general kernel's cluster the whole row some 20.
+    if (ng > (st.mode == kTopK ? kCand / 2 : kCand / 8) && P.vocab > 4 * kCand) {
         leave();
         return;
     }
-    const int qs = gs >> 2, quads = ng * qs;  // four consecutive logits at a time
-#pragma unroll 4
-    for (int q = threadIdx.x; q < quads; q += kThreads) {
-        const int i0 = ((int)S.glist[q / qs] << P.gshift) + (q % qs) * 4;
-        float v[4];
-        if (vec && i0 + 3 < P.vocab) {
-            const float4 f = *reinterpret_cast<const float4*>(row + i0);
-            v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
-        } else {
+    const int qshift = P.gshift - 2, quads = ng << qshift;  // four consecutive logits at a time
+    constexpr int B = 8;                                     // of them per thread in flight
+    for (int q0 = threadIdx.x; q0 < quads; q0 += B * kThreads) {
+        float v[B][4];
+        int at[B];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = i0 + e < P.vocab ? row[i0 + e] : -INFINITY;
+        for (int b = 0; b < B; ++b) {
+            const int q = q0 + b * kThreads;
+            at[b] = q < quads ? ((int)S.glist[q >> qshift] << P.gshift) + (q & ((1 << qshift) - 1)) * 4 : P.vocab;
+            if (vec) {
+                const float4 f = __ldg(reinterpret_cast<const float4*>(row + (at[b] < P.vocab ? at[b] : 0)));
+                v[b][0] = f.x, v[b][1] = f.y, v[b][2] = f.z, v[b][3] = f.w;
+                if (at[b] >= P.vocab) v[b][0] = v[b][1] = v[b][2] = v[b][3] = -INFINITY;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[b][e] = at[b] + e < P.vocab ? __ldg(row + at[b] + e) : -INFINITY;
+            }
+        }
+        if (P.cap > 0.f) {
+#pragma unroll
+            for (int b = 0; b < B; ++b)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[b][e] = softcap(v[b][e], P.cap);
         }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const uint32_t k = logit_key(capped(v[e], P.cap));
-            if (k >= bound) {
-                const int at = atomicAdd(&S.n, 1);
-                if (at < kCand) S.cand[at] = (unsigned long long)k << 32 | (0xffffffffu - (unsigned)(i0 + e));
+        for (int b = 0; b < B; ++b) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t k = logit_key(v[b][e]);
+                if (k >= bound) {
+                    const int i = atomicAdd(&S.n, 1);
+                    if (i < kCand) S.cand[i] = (unsigned long long)k << 32 | (0xffffffffu - (unsigned)(at[b] + e));
+                }
             }
         }
     }
@@ -558,9 +736,13 @@ __global__ void __launch_bounds__(kThreads) sample_finish_kernel(const SamplePar
         leave();
         return;
     }
+    if (n <= kFew) {
+        finish_few(P, S, st, r, n, m, c, u, total, flip, leave);
+        return;
+    }
     int n2 = pow2_at_least(n);
     for (int i = n + threadIdx.x; i < n2; i += kThreads) S.cand[i] = 0ull;
-    block_sort_desc(S.cand, n2);
+    block_sort_desc_any<kCand / kThreads>(S.cand, S.cand2, n2);
     // Ranks 4t .. 4t + 3: weights, their running sum and where it ends the prefix.
     constexpr int E = kCand / kThreads;
     const int limit = st.mode == kTopK ? min(st.k, n) : n;
@@ -568,7 +750,7 @@ __global__ void __launch_bounds__(kThreads) sample_finish_kernel(const SamplePar
 #pragma unroll
     for (int e = 0; e < E; ++e) {
         const int i = threadIdx.x * E + e;
-        w[e] = i < limit ? weight(key_logit((uint32_t)(S.cand[i] >> 32)), m, st.c, S.table) : 0.0;
+        w[e] = i < limit ? weight(key_logit((uint32_t)(S.cand[i] >> 32)), m, c) : 0.0;
         if (i < n2) S.w[i] = w[e];
         own += w[e];
     }
@@ -597,7 +779,7 @@ __global__ void __launch_bounds__(kThreads) sample_finish_kernel(const SamplePar
         // ~index << 32 | position: largest first is lowest index first
         S.cand[i] = i < kept ? (S.cand[i] & 0xffffffffull) << 32 | (unsigned)i : 0ull;
     }
-    block_sort_desc(S.cand, n2);
+    block_sort_desc_any<kCand / kThreads>(S.cand, S.cand2, n2);
     own = 0.0;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
@@ -630,26 +812,30 @@ __global__ void __launch_bounds__(kThreads) sample_finish_kernel(const SamplePar
 // A cluster of up to 16 CTAs takes queued rows, each CTA with its part of the row in shared
 // memory (warps own consecutive segments of 128 * J logits).
 constexpr int kMaxCluster = 16;
-constexpr int kPick = 1024;  // logits ranked at the end of a search
-constexpr int kWays = 8;
+constexpr int kPick = kThreads;  // logits ranked at the end of a search
+constexpr int kWays = 4;
+constexpr int kBins = 256;
 
 struct GeneralShared {
-    double table[32];
     double xd[2][kMaxCluster][kWays];  // per rank: sums of a step
     int xn[2][kMaxCluster][kWays];     // per rank: counts of a step
     uint32_t xlow[kMaxCluster];        // per rank: ~ the lowest key
-    unsigned long long cand[kPick];
+    unsigned long long cand[kPick], cand2[kPick];
     BlockScratch scratch;
     double wsum[kWarps];
     int wcnt[kWarps];
     double red[kWarps][kWays];
     int redn[kWarps][kWays];
-    uint32_t found_key;
-    int found_idx, ncand, work;
+    uint32_t hist[kMaxCluster][kBins];  // per rank: number (at most 49152) and mean place of a part's logits
+    uint32_t own_hist[kBins], own_place[kBins];
+    double above, past_at, n_at, n_b0, n_b1;
+    float found_v;
+    int found_idx, ncand, at, b0, b1, verdict;
 };
-// The kept prefix: keys above `key`, and equal ones up to index `idx`.
+// A kept prefix: logits above v, and equal ones up to index idx.  (Comparisons of floats leave NaN
+// out and take -0 for +0, as the keys do.)
 struct Limit {
-    uint32_t key;
+    float v;
     int idx;
 };
 
@@ -664,28 +850,51 @@ struct General {
     double c;
 
     __device__ int first_index() const { return rank * kThreads * 4 * J; }
-    __device__ bool inside(uint32_t k, int i, const Limit& lim) const {
-        return k != 0u && (k > lim.key || (k == lim.key && i <= lim.idx));
-    }
-    // f(index, logit) over this thread's logits, in the warp's segment.
+    __device__ static bool inside(float v, int i, const Limit& lim) { return v > lim.v || (v == lim.v && i <= lim.idx); }
+    // f(index, four logits from it on) over this thread's logits, in the warp's segment.
     template <class F>
-    __device__ void each(F f) const {
+    __device__ __forceinline__ void each(F f) const {
         const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
         for (int j = 0; j < J; ++j) {
             const int o = (w * J + j) * 128 + lane * 4;
-            const float4 v = *reinterpret_cast<const float4*>(chunk + o);
-            const int i = first_index() + o;
-            f(i, v.x);
-            f(i + 1, v.y);
-            f(i + 2, v.z);
-            f(i + 3, v.w);
+            const float4 q = *reinterpret_cast<const float4*>(chunk + o);
+            const float v[4] = {q.x, q.y, q.z, q.w};
+            f(first_index() + o, v);
         }
     }
-    // Sums over the cluster of kWays doubles and counts per thread (added in rank order).
-    __device__ void cluster_sums(double (&d)[kWays], int (&n)[kWays]) {
+    // The sum of weight over this thread's logits that keep(index, logit) takes.  A bit per logit
+    // first, then only those: of a nucleus of some thousand tokens each thread has a few of 32.
+    template <class K>
+    __device__ __forceinline__ double weigh(K keep) const {
+        const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+        double sum = 0.0;
+        for (int j0 = 0; j0 < J; j0 += 8) {
+            uint32_t bits = 0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                if (j0 + j >= J) break;
+                const int o = (w * J + j0 + j) * 128 + lane * 4;
+                const float4 q = *reinterpret_cast<const float4*>(chunk + o);
+                const float v[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) bits |= (keep(first_index() + o + e, v[e]) ? 1u : 0u) << (j * 4 + e);
+            }
+            while (__any_sync(0xffffffffu, bits != 0u)) {
+                if (bits) {
+                    const int k = __ffs(bits) - 1;
+                    bits &= bits - 1;
+                    sum += weight(chunk[(w * J + j0 + (k >> 2)) * 128 + lane * 4 + (k & 3)], m, c);
+                }
+            }
+        }
+        return sum;
+    }
+    // Sums over the cluster of N doubles and counts per thread (added in rank order).
+    template <int N>
+    __device__ __forceinline__ void cluster_sums(double (&d)[N], int (&n)[N]) {
         const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
 #pragma unroll
-        for (int i = 0; i < kWays; ++i) {
+        for (int i = 0; i < N; ++i) {
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) d[i] += __shfl_xor_sync(0xffffffffu, d[i], o);
             n[i] = __reduce_add_sync(0xffffffffu, n[i]);
@@ -693,42 +902,152 @@ struct General {
         }
         __syncthreads();
         xflip ^= 1;
-        if (threadIdx.x < ranks * kWays) {
-            const int to = threadIdx.x / kWays, i = threadIdx.x % kWays;
-            double s = 0.0;
-            int t = 0;
-            for (int k = 0; k < kWarps; ++k) s += S.red[k][i], t += S.redn[k][i];
-            *cluster.map_shared_rank(&S.xd[xflip][rank][i], to) = s;
-            *cluster.map_shared_rank(&S.xn[xflip][rank][i], to) = t;
+        if (w < N) {  // warp i: value i of the CTA, sent to every rank
+            double s = lane < kWarps ? S.red[lane][w] : 0.0;
+            const int t = __reduce_add_sync(0xffffffffu, lane < kWarps ? S.redn[lane][w] : 0);
+#pragma unroll
+            for (int o = 1; o < kWarps; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+            s = __shfl_sync(0xffffffffu, s, 0);
+            if (lane < ranks) {
+                *cluster.map_shared_rank(&S.xd[xflip][rank][w], lane) = s;
+                *cluster.map_shared_rank(&S.xn[xflip][rank][w], lane) = t;
+            }
         }
         cluster.sync();
 #pragma unroll
-        for (int i = 0; i < kWays; ++i) {
+        for (int i = 0; i < N; ++i) {
             d[i] = 0.0, n[i] = 0;
             for (int k = 0; k < ranks; ++k) d[i] += S.xd[xflip][k][i], n[i] += S.xn[xflip][k][i];
         }
     }
-    __device__ double mass(const Limit& lim, bool count) {
-        double d[kWays] = {};
-        int n[kWays] = {};
-        each([&](int i, float v) {
-            const uint32_t k = logit_key(v);
-            if (inside(k, i, lim)) d[0] += count ? 1.0 : weight(v, m, c, S.table);
-        });
+    // What the logits above `past` inside `lim` weigh, and how many are inside `lim` at all.
+    __device__ double mass(const Limit& lim, float past) {
+        double d[1] = {weigh([&](int i, float v) { return v > past && inside(v, i, lim); })};
+        int n[1] = {0};
         cluster_sums(d, n);
         return d[0];
     }
+    __device__ int number(const Limit& lim) {
+        double d[1] = {0.0};
+        int n[1] = {0};
+        each([&](int i, const float (&v)[4]) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) n[0] += inside(v[e], i + e, lim);
+        });
+        cluster_sums(d, n);
+        return n[0];
+    }
 
-    // The shortest prefix inside `lim` whose weight (number, if count) is at least t.  [lo, hi) are
-    // the keys where it ends, `above` what the keys from hi on weigh; each step cuts them in eight,
-    // in turn evenly in value (which suits what logits look like) and in key (which ends after at
-    // most eleven steps).
+    // The shortest prefix inside `lim` whose weight (or number, if count) is at least t, from
+    // histograms: 256 parts of the keys [lo, hi), even in value, then the parts around the one where
+    // the number (exactly) or the weight (number times the weight in the mean place, some 1e-3 off at
+    // first) passes t, with the exact weight of all above them, until at most kPick logits are left;
+    // those are ranked.  *ok is false where that does not end on the prefix (ties, or a border nearer
+    // than the estimate): search() does then.  Every CTA of the cluster computes the same steps from
+    // the same sums, in one order.
+    __device__ Limit estimate(const Limit& lim, double t, bool count, bool* ok) {
+        uint32_t lo = low, hi = top + 1;
+        double above = 0.0;
+        *ok = false;
+        cluster.sync();  // (a histogram of an earlier call may still be read)
+        for (int step = 0; step < 5; ++step) {
+            const float a = key_logit(lo), b = key_logit(hi - 1);
+            if (!(a > -3.0e38f && b < 3.0e38f && a < b)) return lim;
+            const float scale = (float)kBins / (b - a);
+            if (!(scale < 3.0e38f && scale > 0.f)) return lim;
+            auto bin = [&](float v) { return min(kBins - 1, (int)((v - a) * scale)); };
+            if (threadIdx.x < kBins) S.own_hist[threadIdx.x] = S.own_place[threadIdx.x] = 0;
+            if (threadIdx.x == 0) S.at = -1, S.b0 = kBins, S.b1 = -1;
+            __syncthreads();
+            each([&](int i, const float (&v)[4]) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (v[e] >= a && v[e] <= b && inside(v[e], i + e, lim)) {
+                        const int at = bin(v[e]);
+                        atomicAdd(&S.own_hist[at], 1u);
+                        // its place in the part, in 1/32768
+                        if (!count) atomicAdd(&S.own_place[at], (uint32_t)(((v[e] - a) * scale - (float)at) * 32768.f));
+                    }
+            });
+            if (step > 0) cluster.sync();  // the last step's histograms have been read
+            __syncthreads();
+            if (threadIdx.x < kBins) {
+                const uint32_t n = S.own_hist[threadIdx.x];
+                S.own_hist[threadIdx.x] = n << 16 | (n ? min(S.own_place[threadIdx.x] / n, 65535u) : 0u);
+            }
+            __syncthreads();
+            for (int x = threadIdx.x; x < kBins * ranks; x += kThreads)
+                *cluster.map_shared_rank(&S.hist[rank][x % kBins], x / kBins) = S.own_hist[x % kBins];
+            cluster.sync();
+            // Parts from the top: thread i has part 255 - i.
+            const int q = kBins - 1 - (int)threadIdx.x;
+            uint32_t n = 0;
+            double x = 0.0;
+            if (q >= 0) {
+                float place = 0.f;
+                for (int k = 0; k < ranks; ++k) {
+                    const uint32_t h = S.hist[k][q];
+                    n += h >> 16;
+                    place += (float)(h >> 16) * (float)(h & 65535u);
+                }
+                x = (double)n;
+                if (!count && n) x *= weight(fminf(a + ((float)q + place / (float)n * (1.f / 32768.f)) / scale, m), m, c);
+            }
+            double all;
+            const double before = above + block_prefix(x, S.scratch, flip, &all);
+            const double past = block_prefix((double)n, S.scratch, flip, &all);  // logits in the parts above
+            if (q >= 0 && before < t && before + x >= t) atomicMax(&S.at, q);
+            __syncthreads();
+            const int at = max(S.at, 0);
+            if (q == at) S.past_at = past, S.n_at = (double)n;
+            __syncthreads();
+            // The window: that part, and for an estimate some hundred logits (a part at least) on each side.
+            if (q >= 0) {
+                const double side = count ? -1.0 : kPick / 4;
+                if (q == at || (q > at && S.past_at - past <= side)) atomicMax(&S.b1, q);
+                if (q == at || (q < at && past + n - S.past_at - S.n_at <= side)) atomicMin(&S.b0, q);
+            }
+            __syncthreads();
+            const int b0 = count ? at : max(0, min(S.b0, at - 1)), b1 = count ? at : min(kBins - 1, max(S.b1, at + 1));
+            if (q == b1) S.above = before, S.n_b1 = past;
+            if (q == b0) S.n_b0 = past + n;
+            __syncthreads();
+            above = S.above;
+            const double in = S.n_b0 - S.n_b1;
+            // The keys of the window: the lowest in part b0, the lowest past part b1 (parts rise with the
+            // keys; the searches start next to where the part's border is in value).
+            auto edge = [&](int part) {
+                uint32_t l = lo, h = hi;  // the first key in [l, h] whose part is `part` or more (hi: none)
+                const uint32_t guess = logit_key(fminf(fmaxf(a + part / scale, a), b));
+                const uint32_t g0 = max(guess, lo + 64u) - 64u, g1 = min(guess + 64u, hi - 1);
+                if (bin(key_logit(g0)) < part && bin(key_logit(g1)) >= part) l = g0, h = g1;
+                while (l < h) {
+                    const uint32_t mid = l + ((h - l) >> 1);
+                    if (bin(key_logit(mid)) >= part) h = mid;
+                    else l = mid + 1;
+                }
+                return l;
+            };
+            const uint32_t nlo = b0 > 0 ? edge(b0) : lo, nhi = b1 < kBins - 1 ? edge(b1 + 1) : hi;
+            if (in > (double)kPick && nlo == lo && nhi == hi) return lim;
+            lo = nlo, hi = nhi;
+            if (!count) above = mass(lim, key_logit(hi - 1));
+            if (!(above < t)) return lim;
+            if (in <= (double)kPick) return rank_window(lim, lo, hi, above, t, count, ok);
+        }
+        return lim;
+    }
+
+    // The same by exact sums: [lo, hi) are the keys where the prefix ends, `above` what the keys from
+    // hi on weigh; each step cuts them in four, in turn evenly in value and in key (which ends after
+    // at most sixteen steps).
     __device__ Limit search(const Limit& lim, double t, bool count) {
         uint32_t lo = low, hi = top + 1;
         double above = 0.0;
         int inside_n = 0x7fffffff;
         for (int step = 0; inside_n > kPick && hi - lo > 1; ++step) {
             uint32_t cut[kWays];
+            float cutv[kWays];
             const float a = key_logit(lo), b = key_logit(hi - 1);
             const bool even = (step & 1) == 0 && a > -3.0e38f && b < 3.0e38f && a < b;
 #pragma unroll
@@ -736,16 +1055,27 @@ struct General {
                 uint32_t k = lo + (uint32_t)((unsigned long long)(hi - lo) * i / kWays);
                 if (even && i > 0) k = logit_key((float)((double)a + ((double)b - (double)a) * (i / (double)kWays)));
                 cut[i] = i == 0 ? lo : min(max(k, cut[i - 1]), hi);
+                cutv[i] = cut[i] < hi ? key_logit(cut[i]) : INFINITY;  // (an empty part: at most +inf logits, unused)
             }
             double d[kWays] = {};
             int n[kWays] = {};
-            each([&](int i, float v) {
-                const uint32_t k = logit_key(v);
-                if (k >= lo && k < hi && inside(k, i, lim)) {
-                    const double w = count ? 1.0 : weight(v, m, c, S.table);
+            each([&](int i, const float (&v)[4]) {
+                bool in[4], any = false;
 #pragma unroll
-                    for (int q = 0; q < kWays; ++q)
-                        if (k >= cut[q]) d[q] += w, n[q] += 1;
+                for (int e = 0; e < 4; ++e) {
+                    in[e] = v[e] >= a && v[e] <= b && inside(v[e], i + e, lim);
+                    any = any || in[e];
+                }
+                if (!__any_sync(0xffffffffu, any)) return;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const double w = count ? 1.0 : weight(v[e], m, c);
+#pragma unroll
+                    for (int q = 0; q < kWays; ++q) {
+                        const bool here = in[e] && v[e] >= cutv[q];
+                        d[q] += here ? w : 0.0;
+                        n[q] += here;
+                    }
                 }
             });
             cluster_sums(d, n);
@@ -763,58 +1093,65 @@ struct General {
             }
             lo = nlo, hi = nhi, above = nabove, inside_n = na;
         }
-        if (inside_n > kPick) return nth_equal(lim, lo, above, t, count, inside_n);
-        // Rank what is left in CTA 0.
+        if (inside_n > kPick) return nth_equal(lim, key_logit(lo), above, t, count, inside_n);
+        bool ok;
+        return rank_window(lim, lo, hi, above, t, count, &ok);
+    }
+
+    // Ranks the logits with keys in [lo, hi) (at most kPick) in CTA 0: the end of the shortest prefix
+    // that reaches t, where all keys from hi on weigh `above`.  *ok: there is one.
+    __device__ Limit rank_window(const Limit& lim, uint32_t lo, uint32_t hi, double above, double t, bool count, bool* ok) {
         if (threadIdx.x == 0) S.ncand = 0;
         cluster.sync();
         int* cnt = cluster.map_shared_rank(&S.ncand, 0);
         unsigned long long* list = cluster.map_shared_rank(&S.cand[0], 0);
-        each([&](int i, float v) {
-            const uint32_t k = logit_key(v);
-            if (k >= lo && k < hi && inside(k, i, lim))
-                list[atomicAdd(cnt, 1)] = (unsigned long long)k << 32 | (0xffffffffu - (unsigned)i);
+        const float a = key_logit(lo), b = key_logit(hi - 1);
+        each([&](int i, const float (&v)[4]) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (v[e] >= a && v[e] <= b && inside(v[e], i + e, lim)) {
+                    const int at = atomicAdd(cnt, 1);
+                    if (at < kPick) list[at] = (unsigned long long)logit_key(v[e]) << 32 | (0xffffffffu - (unsigned)(i + e));
+                }
+            }
         });
         cluster.sync();
         if (rank == 0) {
-            const int n = S.ncand, n2 = pow2_at_least(n);
-            for (int i = n + threadIdx.x; i < n2; i += kThreads) S.cand[i] = 0ull;
-            block_sort_desc(S.cand, n2);
-            constexpr int E = kPick / kThreads;
-            double w[E], own = 0.0, all;
-#pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const int i = threadIdx.x * E + e;
-                w[e] = i < n ? (count ? 1.0 : weight(key_logit((uint32_t)(S.cand[i] >> 32)), m, c, S.table)) : 0.0;
-                own += w[e];
-            }
-            double run = above + block_prefix(own, S.scratch, flip, &all);
-            if (threadIdx.x == 0) S.work = n - 1;
+            const int n = min(S.ncand, kPick), n2 = pow2_at_least(n), t0 = threadIdx.x;
+            for (int i = n + t0; i < n2; i += kThreads) S.cand[i] = 0ull;
+            block_sort_desc<1>(S.cand, S.cand2, n2);
+            const double w = t0 >= n ? 0.0 : count ? 1.0 : weight(key_logit((uint32_t)(S.cand[t0] >> 32)), m, c);
+            if (t0 == 0) S.at = n;
+            double all;
+            const double run = above + block_prefix(w, S.scratch, flip, &all) + w;
+            if (t0 < n && run >= t) atomicMin(&S.at, t0);
             __syncthreads();
-#pragma unroll
-            for (int e = 0; e < E; ++e) {
-                run += w[e];
-                if (threadIdx.x * E + e < n && run >= t) atomicMin(&S.work, threadIdx.x * E + e);
-            }
-            __syncthreads();
-            if (threadIdx.x < ranks) {
-                const unsigned long long f = S.cand[S.work];
-                *cluster.map_shared_rank(&S.found_key, threadIdx.x) = (uint32_t)(f >> 32);
-                *cluster.map_shared_rank(&S.found_idx, threadIdx.x) = (int)(0xffffffffu - (unsigned)f);
+            if (t0 < ranks) {
+                const int at = S.at;
+                const unsigned long long f = S.cand[at < n ? at : max(n - 1, 0)];  // the last one, if a rounding left none
+                *cluster.map_shared_rank(&S.found_v, t0) = key_logit((uint32_t)(f >> 32));
+                *cluster.map_shared_rank(&S.found_idx, t0) = (int)(0xffffffffu - (unsigned)f);
+                *cluster.map_shared_rank(&S.verdict, t0) = at < n;
             }
         }
         cluster.sync();
-        return Limit{S.found_key, S.found_idx};
+        *ok = S.verdict != 0;
+        return Limit{S.found_v, S.found_idx};
     }
 
-    // The search ended at one key shared by `n` logits of one weight: the first of them, in index
-    // order, that reach t.
-    __device__ Limit nth_equal(const Limit& lim, uint32_t key, double above, double t, bool count, int n) {
-        const double w = count ? 1.0 : weight(key_logit(key), m, c, S.table);
+    // The search ended at one value shared by `n` logits: the first of them, in index order, that
+    // reach t.
+    __device__ Limit nth_equal(const Limit& lim, float value, double above, double t, bool count, int n) {
+        const double w = count ? 1.0 : weight(value, m, c);
         const double q = ceil((t - above) / w);
         const int need = q >= (double)n ? n : q > 1.0 ? (int)q : 1;
-        double d[kWays] = {};
-        int own[kWays] = {};
-        each([&](int i, float v) { own[0] += logit_key(v) == key && inside(key, i, lim); });
+        double d[1] = {0.0};
+        int own[1] = {0};
+        auto equal = [&](int i, float v) { return v == value && inside(v, i, lim); };
+        each([&](int i, const float (&v)[4]) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) own[0] += equal(i + e, v[e]);
+        });
         const int mine = own[0];
         cluster_sums(d, own);
         int before = 0;
@@ -832,7 +1169,7 @@ struct General {
                     const int o = (w0 * J + j) * 128 + lane * 4, i0 = first_index() + o;
                     int eq[4], cnt = 0;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) cnt += eq[e] = logit_key(chunk[o + e]) == key && inside(key, i0 + e, lim);
+                    for (int e = 0; e < 4; ++e) cnt += eq[e] = equal(i0 + e, chunk[o + e]);
                     int x = cnt;
 #pragma unroll
                     for (int s = 1; s < 32; s <<= 1) {
@@ -851,20 +1188,32 @@ struct General {
             }
         }
         cluster.sync();
-        return Limit{key, S.found_idx};
+        return Limit{value, S.found_idx};
     }
 
     // The pick in index order among what `lim` and mp keep.
     __device__ void pick(const Limit& lim, double mp, double u) {
         const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-        auto kept = [&](int i, float v) {
-            if (!inside(logit_key(v), i, lim)) return 0.0;
-            const double x = weight(v, m, c, S.table);
+        auto kept = [&](float v) {
+            const double x = weight(v, m, c);
             return x < mp ? 0.0 : x;
         };
-        double d[kWays] = {};
-        int n[kWays] = {};
-        each([&](int i, float v) { d[0] += kept(i, v); });
+        // min_p as a value: w rises with the logit
+        float least = lim.v;
+        if (mp > 0.0) {
+            uint32_t lo = kLowestKey, hi = top;
+            while (lo < hi) {
+                const uint32_t span = hi - lo;
+                auto cut = [&](int t) { return lo + (uint32_t)((unsigned long long)span * (unsigned)t / kThreads); };
+                const int below = __syncthreads_count(weight(key_logit(cut(threadIdx.x)), m, c) < mp);
+                const uint32_t nhi = below < kThreads ? cut(below) : hi;
+                lo = below > 0 ? cut(below - 1) + 1 : lo;
+                hi = nhi;
+            }
+            least = key_logit(hi);
+        }
+        double d[1] = {weigh([&](int i, float v) { return v >= least && inside(v, i, lim); })};
+        int n[1] = {0};
         double ws = d[0];
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) ws += __shfl_xor_sync(0xffffffffu, ws, o);
@@ -892,7 +1241,7 @@ struct General {
             const int o = (w * J + j) * 128 + lane * 4, i0 = first_index() + o;
             double x[4], s = 0.0;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s += x[e] = kept(i0 + e, chunk[o + e]);
+            for (int e = 0; e < 4; ++e) s += x[e] = chunk[o + e] >= least && inside(chunk[o + e], i0 + e, lim) ? kept(chunk[o + e]) : 0.0;
             double y = s;
 #pragma unroll
             for (int q = 1; q < 32; q <<= 1) {
@@ -915,14 +1264,13 @@ struct General {
     }
 };
 
-__global__ void __launch_bounds__(kThreads) sample_general_kernel(const SampleParams P, int J) {
+__global__ void __launch_bounds__(kThreads, 2) sample_general_kernel(const SampleParams P, int J, int vec) {
     extern __shared__ __align__(16) uint8_t smem_raw[];
     GeneralShared& S = *reinterpret_cast<GeneralShared*>(smem_raw);
     float* chunk = reinterpret_cast<float*>(smem_raw + ((sizeof(GeneralShared) + 15) & ~size_t(15)));
     cg::cluster_group cluster = cg::this_cluster();
     const int rank = (int)cluster.block_rank(), ranks = (int)cluster.num_blocks();
     pdl_trigger();
-    fill_table(S.table);
     pdl_wait();
     cluster.sync();  // every CTA of the cluster runs before any writes to another's shared memory
     General g{P, S, chunk, cluster, rank, ranks, J, 0, 0, 0, 0.f, 0u, 0u, 0.0};
@@ -932,14 +1280,38 @@ __global__ void __launch_bounds__(kThreads) sample_general_kernel(const SamplePa
         const float* row = P.logits + (size_t)r * P.ld;
         g.r = r;
         __syncthreads();
-        const int i0 = g.first_index(), per = kThreads * 4 * J;
+        const int i0 = g.first_index();
         uint32_t top = 0, low = 0;
-#pragma unroll 8
-        for (int o = threadIdx.x; o < per; o += kThreads) {
-            const float v = i0 + o < P.vocab ? capped(row[i0 + o], P.cap) : -INFINITY;
-            chunk[o] = v;
-            const uint32_t k = logit_key(v);
-            if (k) low = max(low, ~k);
+        constexpr int B = 8;  // loads of a thread in flight
+        for (int j0 = 0; j0 < J; j0 += B) {
+            float4 v[B];
+#pragma unroll
+            for (int b = 0; b < B; ++b) {
+                const int i = i0 + ((j0 + b) * kThreads + threadIdx.x) * 4;
+                v[b] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+                if (vec) {
+                    if (j0 + b < J && i < P.vocab) v[b] = __ldg(reinterpret_cast<const float4*>(row + i));
+                } else if (j0 + b < J) {
+                    if (i < P.vocab) v[b].x = __ldg(row + i);
+                    if (i + 1 < P.vocab) v[b].y = __ldg(row + i + 1);
+                    if (i + 2 < P.vocab) v[b].z = __ldg(row + i + 2);
+                    if (i + 3 < P.vocab) v[b].w = __ldg(row + i + 3);
+                }
+            }
+#pragma unroll
+            for (int b = 0; b < B; ++b) {
+                if (j0 + b >= J) break;
+                if (P.cap > 0.f)
+                    v[b] = make_float4(softcap(v[b].x, P.cap), softcap(v[b].y, P.cap), softcap(v[b].z, P.cap),
+                                       softcap(v[b].w, P.cap));
+                *reinterpret_cast<float4*>(chunk + ((j0 + b) * kThreads + threadIdx.x) * 4) = v[b];
+                const float e[4] = {v[b].x, v[b].y, v[b].z, v[b].w};
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const uint32_t k = logit_key(e[q]);
+                    low = k ? max(low, ~k) : low;
+                }
+            }
         }
         for (int i = threadIdx.x; i < P.groups; i += kThreads) top = max(top, P.gkey[(size_t)r * P.groups + i]);
         g.top = block_max(top, S.scratch, g.flip);  // (its barrier also closes the loads of the chunk)
@@ -951,10 +1323,25 @@ __global__ void __launch_bounds__(kThreads) sample_general_kernel(const SamplePa
         for (int k = 0; k < ranks; ++k) low = max(low, S.xlow[k]);
         g.low = ~low;
         const RowSettings st = row_settings(P, r);
-        g.c = st.c;
-        Limit lim{0u, 0};
-        if (st.k && g.mass(lim, true) > (double)st.k) lim = g.search(lim, (double)st.k, true);
-        if (st.p < 1.0) lim = g.search(lim, st.p * g.mass(lim, false), false);
+        g.c = st.scale();
+        Limit lim{-INFINITY, -1};
+        auto prefix = [&](double t, bool count) {
+            bool ok;
+            const Limit e = g.estimate(lim, t, count, &ok);
+            return ok ? e : g.search(lim, t, count);
+        };
+        if (st.k && g.number(lim) > st.k) lim = prefix((double)st.k, true);
+        if (st.p < 1.0) {
+            double total = 0.0;
+            if (st.k) {
+                total = g.mass(lim, -INFINITY);
+            } else {  // from the groups' weights
+                for (int i = threadIdx.x; i < P.groups; i += kThreads)
+                    total += P.gmass[(size_t)r * P.groups + i] * weight(key_logit(P.gkey[(size_t)r * P.groups + i]), g.m, g.c);
+                total = block_sum(total, S.scratch, g.flip);
+            }
+            lim = prefix(st.p * total, false);
+        }
         g.pick(lim, st.mp, row_uniform(P, r));
         cluster.sync();  // the exchange buffers are free again
     }
@@ -984,12 +1371,14 @@ extern "C" g4_status g4_sample(g4_ctx* ctx, const float* logits, long long ld, i
     P.gkey = reinterpret_cast<uint32_t*>(P.gmass + ng);
     P.queue = reinterpret_cast<int*>(P.gkey + ng);
     const int vec = reinterpret_cast<uintptr_t>(logits) % 16 == 0 && (ld % 4 == 0 || rows == 1);
+    const int vec4 = vec && vocab % 4 == 0;  // every row in whole 16-byte pieces
 
     // The general kernel's cluster: parts of at most 16384 logits if 16 CTAs are enough for that.
     int ranks = 1;
     while (ranks < kMaxCluster && (vocab + ranks - 1) / ranks > 2 * kThreads * 4) ranks <<= 1;
     const int J = (vocab + ranks * kThreads * 4 - 1) / (ranks * kThreads * 4);
     const size_t gsmem = ((sizeof(GeneralShared) + 15) & ~size_t(15)) + (size_t)J * kThreads * 4 * sizeof(float);
+    static_assert(24 * kThreads * 16 + sizeof(GeneralShared) + 16 <= 227 * 1024, "the longest row's parts fit");
     static std::atomic<uint64_t> attr_set{0};
     if (!(attr_set.load() & (1ull << ctx->device))) {
         G4_CHECK_CUDA(cudaFuncSetAttribute(sample_finish_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -1005,12 +1394,12 @@ extern "C" g4_status g4_sample(g4_ctx* ctx, const float* logits, long long ld, i
     const bool pdl = ctx->pdl;
     ctx->pdl = true;
     st = g4::launch(ctx, "sample_finish_kernel", sample_finish_kernel, dim3(rows), dim3(kThreads), sizeof(FinishShared), 1, P,
-                    vec);
+                    vec4);
     // Only top-k, top-p and min-p can leave a row to the general kernel.
     if (!st && (how->top_k || how->top_p || how->min_p)) {
-        const int clusters = std::max(1, std::min(rows, 128 / ranks));
+        const int clusters = std::max(1, std::min(rows, 288 / ranks));
         st = g4::launch(ctx, "sample_general_kernel", sample_general_kernel, dim3(clusters * ranks), dim3(kThreads), gsmem,
-                        ranks, P, J);
+                        ranks, P, J, vec4);
     }
     ctx->pdl = pdl;
     return st;

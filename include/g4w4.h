@@ -369,7 +369,8 @@ typedef struct {
     const float* uniform;      /* required: the row's random number in [0, 1) (others clamped)  */
 } g4_sampling;
 /* One token per row of f32 logits [rows, ld] (ld >= vocab).  With cap > 0 the logits are first
- * capped as g4_softcap does (the same bits as g4_softcap in place, then this call with cap 0).
+ * capped as g4_softcap does (the same bits as g4_softcap in place, then this call with cap 0, but
+ * for -inf logits: a mask stays a mask).
  * NaN and -inf logits are never picked.  The others are ranked by (logit descending, index
  * ascending) and weigh w = exp((logit - highest) / temperature); +inf logits share the whole
  * weight.  Kept is a prefix of the ranking, the shortest of

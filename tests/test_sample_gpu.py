@@ -107,6 +107,10 @@ def test_every_setting_at_its_edges(ops):
     l, _ = rows(40, 2000, 4)
     u = np.linspace(0, 1, 40).astype(np.float32)
     check(ops, l, u, T=np.resize([0.0, -1.0, np.nan, 1e-30, 1e-3, 1e30, np.inf, 1.0], 40))
+    # temperatures at which (logit - highest) / T passes 2^31, 2^32 and 2^33
+    check(ops, l, u, T=np.resize([1e-7, 2e-9, 1e-9, 5e-10, 3e-10, 1e-10], 40))
+    check(ops, l, u, T=np.resize([1e-7, 2e-9, 1e-9, 5e-10, 3e-10, 1e-10], 40), mp=1e-6)
+    check(ops, l, u, T=np.resize([1e-7, 2e-9, 1e-9, 5e-10, 3e-10, 1e-10], 40), p=0.99)
     check(ops, l, u, k=np.resize([-5, 0, 1, 2, 1023, 1024, 1025, 1999, 2000, 2**31 - 1], 40))
     check(ops, l, u, p=np.resize([-1.0, 0.0, 1e-7, 0.5, 0.999999, 1.0, 2.0, np.nan], 40).astype(np.float32))
     check(ops, l, u, mp=np.resize([-1.0, 0.0, 1e-7, 0.3, 1.0, 5.0, np.nan], 40).astype(np.float32))
@@ -182,6 +186,20 @@ def test_cap_is_softcap_first(rt, ctx, ops):
     rt.call("g4_softcap", ctx.handle, C.c_void_p(x.data_ptr()), x.numel(), C.c_float(30.0))
     for a, b in ((got, ops.sample(x, U, top_k=k)), (full, ops.sample(x, U))):
         assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+@pytest.mark.parametrize("V", [3, 130, 4099, 9001])
+def test_cap_keeps_masks_and_the_end_of_the_row(ops, V):
+    """A -inf logit stays unpickable under a cap (g4_softcap would make it -cap), and nothing behind
+    the row becomes a candidate, whatever the settings ask for."""
+    l = np.full((6, V), -np.inf, np.float32)
+    l[:, 0] = [5.0, -50.0, -1000.0, 0.0, -np.inf, 300.0]
+    x = torch.from_numpy(l).cuda()
+    u = torch.full((6,), 0.999999, device="cuda")
+    k, p, mp = torch.full((6,), V - 1, dtype=torch.int32, device="cuda"), torch.full((6,), 0.9, device="cuda"), torch.full((6,), 1e-3, device="cuda")
+    for kw in ({}, {"top_k": k}, {"top_p": p}, {"min_p": mp}, {"top_k": k, "top_p": p, "min_p": mp}):
+        ids, probs = ops.sample(x, u, cap=30.0, **kw)
+        assert ids.tolist() == [0, 0, 0, 0, -1, 0] and probs.tolist() == [1, 1, 1, 1, 0, 1]
 
 
 def test_distribution_of_many_draws(ops):
