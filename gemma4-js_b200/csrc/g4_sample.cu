@@ -43,6 +43,7 @@ struct SampleParams {
     float* probs;
     uint32_t* gkey;   // [rows][groups] highest key of each group
     double* gmass;    // [rows][groups] sum of exp((l - group's highest) / T)
+    double* rowmass;  // [rows] weight of the whole row, for rows left to the general kernel with a top_p and no top_k
     int* queue;       // [0] rows left to the general kernel, then the rows
     int gshift, groups;
 };
@@ -243,6 +244,74 @@ __global__ void __launch_bounds__(kSumWarps * 32) sample_summary_kernel(const Sa
     }
 }
 
+// The same for rows in 16-byte pieces and groups of 128 logits or more (vocabularies above 131072):
+// a warp walks `blocks` blocks of 512 with the next one's loads in flight, and the four chunks'
+// sums are reduced together (12 shuffles of a double where one after the other they take 40).
+__global__ void __launch_bounds__(kSumWarps * 32) sample_summary_wide_kernel(const SampleParams P, int segments, int blocks) {
+    pdl_trigger();
+    pdl_wait();
+    if (blockIdx.x == 0 && threadIdx.x == 0) P.queue[0] = 0;
+    const int lane = threadIdx.x & 31;
+    const int r = (int)(blockIdx.x / (unsigned)segments);
+    const int warp = (int)(blockIdx.x - (unsigned)r * segments) * kSumWarps + (threadIdx.x >> 5);
+    const float* row = P.logits + (size_t)r * P.ld;
+    float4 next[4];
+    auto load = [&](int base) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int at = base + i * 128 + lane * 4;
+            next[i] = at < P.vocab ? __ldg(reinterpret_cast<const float4*>(row + at))
+                                   : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+        }
+    };
+    int base = warp * blocks * 512;
+    if (base >= P.vocab) return;
+    load(base);
+    const RowSettings st = row_settings(P, r);
+    const bool mass = st.mode == kAll || st.mode == kTopP;
+    const double c = mass ? st.scale() : 0.0;
+    for (int k = 0; k < blocks && base < P.vocab; ++k, base += 512) {
+        float v[4][4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i][0] = next[i].x, v[i][1] = next[i].y, v[i][2] = next[i].z, v[i][3] = next[i].w;
+        if (k + 1 < blocks) load(base + 512);
+        if (P.cap > 0.f) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[i][e] = softcap(v[i][e], P.cap);
+        }
+        uint32_t key[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)  // fmaxf passes over NaN
+            key[i] = __reduce_max_sync(0xffffffffu, logit_key(fmaxf(fmaxf(v[i][0], v[i][1]), fmaxf(v[i][2], v[i][3]))));
+        if (P.gshift >= 8) key[0] = key[1] = max(key[0], key[1]), key[2] = key[3] = max(key[2], key[3]);
+        if (P.gshift >= 9) key[0] = key[1] = key[2] = key[3] = max(key[0], key[2]);
+        // Lane 8 i speaks for chunk i.
+        const int i = lane >> 3, g = (base + i * 128) >> P.gshift;
+        const bool writes = (lane & 7) == 0 && ((base + i * 128) & ((1 << P.gshift) - 1)) == 0 && g < P.groups;
+        if (writes) P.gkey[(size_t)r * P.groups + g] = i < 2 ? (i == 0 ? key[0] : key[1]) : (i == 2 ? key[2] : key[3]);
+        if (!mass) continue;
+        double s[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const float m = key_logit(key[q]);  // a group without any: NaN, and all weights 0
+            s[q] = (weight(v[q][0], m, c) + weight(v[q][1], m, c)) + (weight(v[q][2], m, c) + weight(v[q][3], m, c));
+        }
+        const bool hi = lane & 16, odd = lane & 8;
+        double a = hi ? s[2] : s[0], b = hi ? s[3] : s[1];
+        a += __shfl_xor_sync(0xffffffffu, hi ? s[0] : s[2], 16);
+        b += __shfl_xor_sync(0xffffffffu, hi ? s[1] : s[3], 16);
+        double t = odd ? b : a;
+        t += __shfl_xor_sync(0xffffffffu, odd ? a : b, 8);
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+        if (P.gshift >= 8) t += __shfl_xor_sync(0xffffffffu, t, 8);
+        if (P.gshift >= 9) t += __shfl_xor_sync(0xffffffffu, t, 16);
+        if (writes) P.gmass[(size_t)r * P.groups + g] = t;
+    }
+}
+
 // ------------------------------------------------- block-wide building blocks --
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
@@ -389,6 +458,24 @@ struct FinishShared {
     int rank[kFew];
 };
 
+// Lists the logits of four that are `least` or more.  Out of line: code that runs once costs its
+// fetches, not its instructions.
+__device__ __noinline__ void append_quad(FinishShared& S, float4 f, int at, float least, float cap) {
+    float v[4] = {f.x, f.y, f.z, f.w};
+    if (cap > 0.f) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = softcap(v[e], cap);
+    }
+    if (!(v[0] >= least || v[1] >= least || v[2] >= least || v[3] >= least)) return;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        if (v[e] >= least) {
+            const int i = atomicAdd(&S.n, 1);
+            if (i < kCand) S.cand[i] = (unsigned long long)logit_key(v[e]) << 32 | (0xffffffffu - (unsigned)(at + e));
+        }
+    }
+}
+
 // The end of a row with at most kFew candidates: ranks by counting (several threads per candidate)
 // instead of sorts, whose 28 barriers for 128 candidates cost 6400 clocks.
 template <class Leave>
@@ -416,7 +503,7 @@ __device__ __forceinline__ void finish_few(const SampleParams& P, FinishShared& 
     if (st.mode != kTopP) total = all;
     const double need = st.p * total;
     if (st.mode == kTopP && all < need) {
-        leave();
+        leave(total);
         return;
     }
     // kept: the shortest prefix of the filters.
@@ -486,11 +573,11 @@ __global__ void __launch_bounds__(kThreads) sample_finish_kernel(const SamplePar
     }
     const float m = key_logit(top);
     const double u = row_uniform(P, r);
-    auto leave = [&]() {  // to the general kernel
-        if (threadIdx.x == 0) P.queue[1 + atomicAdd(P.queue, 1)] = r;
+    auto leave = [&](double mass) {  // to the general kernel
+        if (threadIdx.x == 0) P.rowmass[r] = mass, P.queue[1 + atomicAdd(P.queue, 1)] = r;
     };
     if (st.mode == kGeneral) {
-        leave();
+        leave(0.0);
         return;
     }
     if (st.mode == kAll) {
@@ -608,7 +695,7 @@ __global__ void __launch_bounds__(kThreads) sample_finish_kernel(const SamplePar
             total = block_sum(own, S.scratch, flip);
             const double fixed = st.p * total * 1048576.0 + kMaxGroups;
             if (fixed > 2147483648.0) {  // more than all maxima can weigh
-                leave();
+                leave(total);
                 return;
             }
             need = (uint32_t)fixed;
@@ -678,7 +765,7 @@ __global__ void __launch_bounds__(kThreads) sample_finish_kernel(const SamplePar
             if (shift == 0 || above + S.found_in <= need + need / 8 + (st.mode == kTopK ? 4 : 0)) done = true;
         }
         if (!enough && st.mode == kTopP) {
-            leave();
+            leave(total);
             return;
         }
         bound = enough ? lo : 1u;
@@ -691,49 +778,37 @@ __global__ void __launch_bounds__(kThreads) sample_finish_kernel(const SamplePar
     // Too many to read here (a short row is tried whole): by one CTA 1024 groups take 60 us, by the
     // general kernel's cluster the whole row some 20.
     if (ng > (st.mode == kTopK ? kCand / 2 : kCand / 8) && P.vocab > 4 * kCand) {
-        leave();
+        leave(total);
         return;
     }
     const int qshift = P.gshift - 2, quads = ng << qshift;  // four consecutive logits at a time
-    constexpr int B = 8;                                     // of them per thread in flight
-    for (int q0 = threadIdx.x; q0 < quads; q0 += B * kThreads) {
-        float v[B][4];
-        int at[B];
-#pragma unroll
-        for (int b = 0; b < B; ++b) {
-            const int q = q0 + b * kThreads;
-            at[b] = q < quads ? ((int)S.glist[q >> qshift] << P.gshift) + (q & ((1 << qshift) - 1)) * 4 : P.vocab;
-            if (vec) {
-                const float4 f = __ldg(reinterpret_cast<const float4*>(row + (at[b] < P.vocab ? at[b] : 0)));
-                v[b][0] = f.x, v[b][1] = f.y, v[b][2] = f.z, v[b][3] = f.w;
-                if (at[b] >= P.vocab) v[b][0] = v[b][1] = v[b][2] = v[b][3] = -INFINITY;
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[b][e] = at[b] + e < P.vocab ? __ldg(row + at[b] + e) : -INFINITY;
-            }
+    const float least = key_logit(max(bound, kLowestKey));  // (NaN compares false)
+    auto place = [&](int q) { return ((int)S.glist[q >> qshift] << P.gshift) + (q & ((1 << qshift) - 1)) * 4; };
+    auto fetch = [&](int at) {
+        float4 f = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+        if (vec) {
+            if (at < P.vocab) f = __ldg(reinterpret_cast<const float4*>(row + at));
+        } else {
+            if (at < P.vocab) f.x = __ldg(row + at);
+            if (at + 1 < P.vocab) f.y = __ldg(row + at + 1);
+            if (at + 2 < P.vocab) f.z = __ldg(row + at + 2);
+            if (at + 3 < P.vocab) f.w = __ldg(row + at + 3);
         }
-        if (P.cap > 0.f) {
-#pragma unroll
-            for (int b = 0; b < B; ++b)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[b][e] = softcap(v[b][e], P.cap);
-        }
-#pragma unroll
-        for (int b = 0; b < B; ++b) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const uint32_t k = logit_key(v[b][e]);
-                if (k >= bound) {
-                    const int i = atomicAdd(&S.n, 1);
-                    if (i < kCand) S.cand[i] = (unsigned long long)k << 32 | (0xffffffffu - (unsigned)(at[b] + e));
-                }
-            }
-        }
+        return f;
+    };
+#pragma unroll 1
+    for (int q = threadIdx.x; q < quads; q += 3 * kThreads) {  // three in flight
+        const int q1 = q + kThreads, q2 = q1 + kThreads;
+        const int a0 = place(q), a1 = q1 < quads ? place(q1) : P.vocab, a2 = q2 < quads ? place(q2) : P.vocab;
+        const float4 f0 = fetch(a0), f1 = fetch(a1), f2 = fetch(a2);
+        append_quad(S, f0, a0, least, P.cap);
+        append_quad(S, f1, a1, least, P.cap);
+        append_quad(S, f2, a2, least, P.cap);
     }
     __syncthreads();
     const int n = S.n;
     if (n > kCand) {
-        leave();
+        leave(total);
         return;
     }
     if (n <= kFew) {
@@ -758,7 +833,7 @@ __global__ void __launch_bounds__(kThreads) sample_finish_kernel(const SamplePar
     if (st.mode != kTopP) total = all;
     const double need = st.p * total;
     if (st.mode == kTopP && all < need) {
-        leave();
+        leave(total);
         return;
     }
     // kept: the longest prefix that the filters leave.
@@ -1003,7 +1078,7 @@ struct General {
             __syncthreads();
             // The window: that part, and for an estimate some hundred logits (a part at least) on each side.
             if (q >= 0) {
-                const double side = count ? -1.0 : kPick / 4;
+                const double side = count ? -1.0 : step == 0 ? kPick / 4 : kPick / 10;
                 if (q == at || (q > at && S.past_at - past <= side)) atomicMax(&S.b1, q);
                 if (q == at || (q < at && past + n - S.past_at - S.n_at <= side)) atomicMin(&S.b0, q);
             }
@@ -1117,9 +1192,28 @@ struct General {
         });
         cluster.sync();
         if (rank == 0) {
-            const int n = min(S.ncand, kPick), n2 = pow2_at_least(n), t0 = threadIdx.x;
-            for (int i = n + t0; i < n2; i += kThreads) S.cand[i] = 0ull;
-            block_sort_desc<1>(S.cand, S.cand2, n2);
+            const int n = min(S.ncand, kPick), t0 = threadIdx.x;
+            if (t0 < n) S.own_hist[t0 & (kBins - 1)] = 0;
+            __syncthreads();
+            if (n <= kBins) {  // ranks by counting, two threads per logit
+                const int i = t0 & (kBins - 1);
+                int over = 0;
+                if (i < n) {
+                    const unsigned long long me = S.cand[i];
+#pragma unroll 4
+                    for (int j = t0 >> 8; j < n; j += 2) over += S.cand[j] > me;
+                    atomicAdd(&S.own_hist[i], (uint32_t)over);
+                }
+                __syncthreads();
+                if (t0 < n) S.cand2[S.own_hist[t0]] = S.cand[t0];
+                __syncthreads();
+                if (t0 < n) S.cand[t0] = S.cand2[t0];
+                __syncthreads();
+            } else {
+                const int n2 = pow2_at_least(n);
+                for (int i = n + t0; i < n2; i += kThreads) S.cand[i] = 0ull;
+                block_sort_desc<1>(S.cand, S.cand2, n2);
+            }
             const double w = t0 >= n ? 0.0 : count ? 1.0 : weight(key_logit((uint32_t)(S.cand[t0] >> 32)), m, c);
             if (t0 == 0) S.at = n;
             double all;
@@ -1335,10 +1429,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_general_kernel(const Sampl
             double total = 0.0;
             if (st.k) {
                 total = g.mass(lim, -INFINITY);
-            } else {  // from the groups' weights
-                for (int i = threadIdx.x; i < P.groups; i += kThreads)
-                    total += P.gmass[(size_t)r * P.groups + i] * weight(key_logit(P.gkey[(size_t)r * P.groups + i]), g.m, g.c);
-                total = block_sum(total, S.scratch, g.flip);
+            } else {
+                total = P.rowmass[r];
             }
             lim = prefix(st.p * total, false);
         }
@@ -1358,17 +1450,18 @@ extern "C" g4_status g4_sample(g4_ctx* ctx, const float* logits, long long ld, i
         return g4::set_error(G4_ERR_INVALID, "g4_sample: null argument");
     g4_status st = g4::use_device(ctx);
     if (st || rows == 0) return st;
-    SampleParams P{logits, ld, rows, vocab, cap, *how, ids_out, probs_out, nullptr, nullptr, nullptr, 2, 0};
+    SampleParams P{logits, ld, rows, vocab, cap, *how, ids_out, probs_out, nullptr, nullptr, nullptr, nullptr, 2, 0};
     while (((vocab + (1 << P.gshift) - 1) >> P.gshift) > kMaxGroups) ++P.gshift;
     P.groups = (vocab + (1 << P.gshift) - 1) >> P.gshift;
     const long long segments = (vocab + kSumWarps * 512 - 1) / (kSumWarps * 512);
     if (segments * rows > 0x7fffffffLL)
         return g4::set_error(G4_ERR_UNSUPPORTED, "g4_sample: %d rows of %d logits", rows, vocab);
     const size_t ng = (size_t)rows * P.groups;
-    st = g4::ensure_workspace(ctx, ng * sizeof(double) + ng * sizeof(uint32_t) + ((size_t)rows + 1) * sizeof(int));
+    st = g4::ensure_workspace(ctx, (ng + rows) * sizeof(double) + ng * sizeof(uint32_t) + ((size_t)rows + 1) * sizeof(int));
     if (st) return st;
     P.gmass = static_cast<double*>(ctx->ws);
-    P.gkey = reinterpret_cast<uint32_t*>(P.gmass + ng);
+    P.rowmass = P.gmass + ng;
+    P.gkey = reinterpret_cast<uint32_t*>(P.rowmass + rows);
     P.queue = reinterpret_cast<int*>(P.gkey + ng);
     const int vec = reinterpret_cast<uintptr_t>(logits) % 16 == 0 && (ld % 4 == 0 || rows == 1);
     const int vec4 = vec && vocab % 4 == 0;  // every row in whole 16-byte pieces
@@ -1387,8 +1480,17 @@ extern "C" g4_status g4_sample(g4_ctx* ctx, const float* logits, long long ld, i
         G4_CHECK_CUDA(cudaFuncSetAttribute(sample_general_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
         attr_set.fetch_or(1ull << ctx->device);
     }
-    st = g4::launch(ctx, "sample_summary_kernel", vec ? sample_summary_kernel<true> : sample_summary_kernel<false>,
-                    dim3((unsigned)(segments * rows)), dim3(kSumWarps * 32), 0, 1, P, (int)segments);
+    if (vec4 && P.gshift >= 7) {
+        // Blocks per warp: up to four, while some eight waves of warps are left.
+        const long long all = (long long)rows * ((vocab + 511) / 512);
+        const int blocks = (int)std::max<long long>(1, std::min<long long>(4, all / (ctx->num_sms * 48 * 2)));
+        const int seg = (vocab + kSumWarps * 512 * blocks - 1) / (kSumWarps * 512 * blocks);
+        st = g4::launch(ctx, "sample_summary_wide_kernel", sample_summary_wide_kernel, dim3((unsigned)((long long)seg * rows)),
+                        dim3(kSumWarps * 32), 0, 1, P, seg, blocks);
+    } else {
+        st = g4::launch(ctx, "sample_summary_kernel", vec ? sample_summary_kernel<true> : sample_summary_kernel<false>,
+                        dim3((unsigned)(segments * rows)), dim3(kSumWarps * 32), 0, 1, P, (int)segments);
+    }
     if (st) return st;
     // The two that follow are set up while their predecessor runs, and wait for it (griddepcontrol).
     const bool pdl = ctx->pdl;
