@@ -522,6 +522,7 @@ g4_status g4_kv_create(g4_ctx* ctx, int hd, int capacity, g4_kv** out) {
     if (capacity <= 0) return g4::set_error(G4_ERR_INVALID, "g4_kv_create: capacity %d", capacity);
     g4_kv* kv = new g4_kv();
     kv->ctx = ctx;
+    kv->device = ctx->device;
     kv->hd = hd;
     kv->capacity = capacity;
     kv->rows_total = capacity;
@@ -561,6 +562,7 @@ g4_status g4_kv_create_ring(g4_ctx* ctx, int hd, int capacity, int ring, int nse
         return g4::set_error(G4_ERR_RANGE, "g4_kv_create_ring: %d sequences x %d rows", nseq, ring + mirror);
     g4_kv* kv = new g4_kv();
     kv->ctx = ctx;
+    kv->device = ctx->device;
     kv->hd = hd;
     kv->capacity = capacity;
     kv->ring = ring;
@@ -596,11 +598,8 @@ g4_status g4_kv_layout(const g4_kv* kv, int* ring, int* seq_rows, int* nseq) {
 
 g4_status g4_kv_destroy(g4_kv* kv) {
     if (!kv) return G4_OK;
-    if (kv->ctx) {
-        cudaSetDevice(kv->ctx->device);
-        cudaStreamSynchronize(kv->ctx->stream);
-    }
-    cudaFree(kv->k);
+    cudaSetDevice(kv->device);
+    cudaFree(kv->k);  // waits for the device's work, this cache's included
     cudaFree(kv->v);
     delete kv;
     return G4_OK;

@@ -11,6 +11,7 @@
 // at the wrap).  mirror = 16384 / hd, the widest key tile of the attention kernels.
 struct g4_kv {
     g4_ctx* ctx = nullptr;
+    int device = 0;             // of ctx, which may be destroyed before the cache
     int hd = 0, capacity = 0, length = 0;
     int rows_total = 0;         // rows covered by the tensor maps
     int ring = 0;               // 0: linear; > 0: slots per sequence

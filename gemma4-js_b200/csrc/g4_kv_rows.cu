@@ -192,9 +192,9 @@ g4_status check_caches(const char* name, const g4_ctx* ctx, g4_kv* const* kvs, i
     for (int i = 0; i < nkv; ++i) {
         const g4_kv* kv = kvs[i];
         if (!kv) return g4::set_error(G4_ERR_INVALID, "%s: null cache %d", name, i);
-        if (kv->ctx->device != ctx->device)
+        if (kv->device != ctx->device)
             return g4::set_error(G4_ERR_INVALID, "%s: cache %d is on device %d, the context on %d", name, i,
-                                 kv->ctx->device, ctx->device);
+                                 kv->device, ctx->device);
         for (int j = 0; j < i; ++j)
             if (kvs[j] == kv) return g4::set_error(G4_ERR_INVALID, "%s: caches %d and %d are the same", name, j, i);
         const int stride = kv->ring ? kv->seq_rows : seq_stride;

@@ -719,9 +719,9 @@ extern "C" g4_status g4_attention_tree(g4_ctx* ctx, const void* q_bf16, const g4
     st = g4::use_device(ctx);
     if (st) return st;
     if (hd != kv->hd) return g4::set_error(G4_ERR_INVALID, "g4_attention_tree: hd %d != cache hd %d", hd, kv->hd);
-    if (kv->ctx->device != ctx->device)
+    if (kv->device != ctx->device)
         return g4::set_error(G4_ERR_INVALID, "g4_attention_tree: the cache is on device %d, the context on %d",
-                             kv->ctx->device, ctx->device);
+                             kv->device, ctx->device);
     if (kv->ring && seq_stride != kv->seq_rows)
         return g4::set_error(G4_ERR_INVALID, "g4_attention_tree: seq_stride %d of a ring cache must be its %d rows per "
                              "sequence", seq_stride, kv->seq_rows);

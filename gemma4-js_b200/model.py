@@ -29,8 +29,8 @@ import numpy as np
 import torch
 
 from . import _lib
-from ._lib import G4Planes, G4Rows, call
-from .runtime import Context, G4Error, KVCache, PleW4Table, W4Linear
+from ._lib import G4Planes, G4Rows, G4Sampling, G4Tree, call
+from .runtime import Context, G4Error, GPUOps, KVCache, PleW4Table, W4Linear, kv_compact, kv_fork
 
 
 @dataclass(frozen=True)
@@ -277,6 +277,28 @@ class Decoder:
             pass
 
 
+@dataclass
+class Sampling:
+    """Settings of sampled decoding: device tensors of one entry per row (f32; top_k int32), None =
+    off (g4_sampling).  `uniform` holds the rows' random numbers in [0, 1) of the next step; a
+    captured step reads them, and every other setting, at each replay."""
+    uniform: torch.Tensor
+    temperature: torch.Tensor | None = None
+    top_k: torch.Tensor | None = None
+    top_p: torch.Tensor | None = None
+    min_p: torch.Tensor | None = None
+
+    def struct(self, rows: int) -> G4Sampling:
+        p = []
+        for name in ("temperature", "top_k", "top_p", "min_p", "uniform"):
+            t = getattr(self, name)
+            want = torch.int32 if name == "top_k" else torch.float32
+            if t is not None and (t.dtype != want or not t.is_cuda or not t.is_contiguous() or t.numel() < rows):
+                raise G4Error(-1, f"sampling: {name} must be a contiguous {want} device tensor of {rows} rows")
+            p.append(None if t is None else t.data_ptr())
+        return G4Sampling(*p)
+
+
 class Gemma4Model:
     """Mirror of Gemma4WebGPU over libg4w4 (see the module docstring).
 
@@ -330,6 +352,7 @@ class Gemma4Model:
         self._alloc(self.max_rows)
         self.graph = None
         self._capturing = False
+        self.ops = GPUOps(ctx)
 
     def _cache(self, spec: dict, ring_kv: bool) -> KVCache:
         """A layer's cache: a ring of window + max_rows - 1 slots per sequence for a sliding
@@ -387,9 +410,17 @@ class Gemma4Model:
         call("g4_linear_w4a16_planes", self.ctx.handle, lin.handle, _ptr(x), rows, C.byref(pl))
         return pl
 
-    def _forward(self, ids, rows, rmap: G4Rows, head_rows: int, head_x_row0: int):
-        """Issues one forward of `rows` rows (ids: int32 device [rows]) and the greedy pick
-        of `head_rows` rows starting at row head_x_row0 into buf["next"]."""
+    def _forward(self, ids, rows, rmap: G4Rows, head_rows: int, head_x_row0: int,
+                 sampling: Sampling | None = None):
+        """Issues one forward of `rows` rows (ids: int32 device [rows]) and the pick of
+        `head_rows` rows starting at row head_x_row0 into buf["next"]: the greedy one, or a
+        sampled one."""
+        self._layers(ids, rows, rmap)
+        b = self.buf
+        self._pick(b["x"][head_x_row0:head_x_row0 + head_rows], head_rows, b["next"], b["val"], b["logits"], sampling)
+
+    def _layers(self, ids, rows, rmap: G4Rows, tree: G4Tree | None = None):
+        """Embedding to final norm of `rows` rows; with a tree, they are the nodes of drafted trees."""
         cfg, b, h = self.cfg, self.buf, self.ctx.handle
         H, P, L = cfg.hidden, cfg.ple_dim, cfg.layers
         # inputBuffers + top-level embedding and PLE projection (gemma4-webgpu.js:198-213, :316-323)
@@ -408,7 +439,11 @@ class Gemma4Model:
             kp, vp = C.c_void_p(), C.c_void_p()
             call("g4_kv_buffers", kv.handle, C.byref(kp), C.byref(vp))
             qkv = self._w4p(Ly["qkv"], b["x"], rows)
-            if kv.ring and not s["shared"]:
+            if tree is not None:
+                call("g4_qkv_post_tree", h, C.byref(qkv), cfg.heads, hd, _ptr(Ly["qn"]), _ptr(Ly["kn"]),
+                     C.c_float(cfg.eps), s["rope_angles"], C.c_float(s["rope_base"]), C.byref(rmap), C.byref(tree), rows,
+                     _ptr(b["q"]), None if s["shared"] else kv.handle, self.max_seq)
+            elif kv.ring and not s["shared"]:
                 call("g4_qkv_post_kv", h, C.byref(qkv), cfg.heads, hd, _ptr(Ly["qn"]), _ptr(Ly["kn"]),
                      C.c_float(cfg.eps), s["rope_angles"], C.c_float(s["rope_base"]), C.byref(rmap), rows,
                      _ptr(b["q"]), kv.handle)
@@ -416,8 +451,12 @@ class Gemma4Model:
                 call("g4_qkv_post_planes", h, C.byref(qkv), cfg.heads, hd, 0 if s["shared"] else 1,
                      _ptr(Ly["qn"]), _ptr(Ly["kn"]), C.c_float(cfg.eps), s["rope_angles"], C.c_float(s["rope_base"]),
                      C.byref(rmap), rows, _ptr(b["q"]), kp, vp, self.max_seq)
-            call("g4_attention_rows", h, _ptr(b["q"]), kv.handle, rows, cfg.heads, hd, C.byref(rmap), self.kv_stride(kv),
-                 0 if s["full"] else 1, cfg.window, _ptr(b["attn"]))
+            if tree is not None:
+                call("g4_attention_tree", h, _ptr(b["q"]), kv.handle, rows, cfg.heads, hd, C.byref(rmap), C.byref(tree),
+                     self.kv_stride(kv), 0 if s["full"] else 1, cfg.window, _ptr(b["attn"]))
+            else:
+                call("g4_attention_rows", h, _ptr(b["q"]), kv.handle, rows, cfg.heads, hd, C.byref(rmap),
+                     self.kv_stride(kv), 0 if s["full"] else 1, cfg.window, _ptr(b["attn"]))
             y = self._w4p(Ly["o"], b["attn"], rows)
             call("g4_post_norm_add_planes", h, _ptr(b["h"]), C.byref(y), _ptr(Ly["n_pa"]), C.c_float(1.0),
                  _ptr(Ly["n_pf"]), rows, H, C.c_float(cfg.eps), _ptr(b["x"]))
@@ -432,19 +471,24 @@ class Gemma4Model:
             w_next = self.layers[i + 1]["n_in"] if i + 1 < L else self.final_norm  # :404 final rms fused here
             call("g4_post_norm_add_planes", h, _ptr(b["h"]), C.byref(y), _ptr(Ly["n_pple"]), C.c_float(Ly["skip"]),
                  _ptr(w_next), rows, H, C.c_float(cfg.eps), _ptr(b["x"]))
-        # logits + greedy (gemma4-webgpu.js:413-480)
-        xh = b["x"][head_x_row0:head_x_row0 + head_rows]
-        if head_rows > 16:  # batched: logits tiles reduced in the head kernel's epilogue, never stored
-            call("g4_dense_argmax", h, self.head.handle, _ptr(xh), head_rows, C.c_float(cfg.softcap), _ptr(b["next"]),
-                 _ptr(b["val"]))
-        else:
-            call("g4_dense_matmul", h, self.head.handle, _ptr(xh), head_rows, _ptr(b["logits"]))
-            call("g4_softcap_argmax", h, _ptr(b["logits"]), head_rows, cfg.vocab, C.c_float(cfg.softcap),
-                 _ptr(b["next"]), _ptr(b["val"]))
 
-    def prefill(self, seq: int, ids) -> int:
+    def _pick(self, xh, rows: int, ids, vals, logits, sampling: Sampling | None):
+        """logits + greedy (gemma4-webgpu.js:413-480), or g4_sample of the capped logits."""
+        cfg, h = self.cfg, self.ctx.handle
+        if sampling is not None:
+            how = sampling.struct(rows)
+            call("g4_dense_matmul", h, self.head.handle, _ptr(xh), rows, _ptr(logits))
+            call("g4_sample", h, _ptr(logits), cfg.vocab, rows, cfg.vocab, C.c_float(cfg.softcap), C.byref(how), _ptr(ids),
+                 _ptr(vals))
+        elif rows > 16:  # batched: logits tiles reduced in the head kernel's epilogue, never stored
+            call("g4_dense_argmax", h, self.head.handle, _ptr(xh), rows, C.c_float(cfg.softcap), _ptr(ids), _ptr(vals))
+        else:
+            call("g4_dense_matmul", h, self.head.handle, _ptr(xh), rows, _ptr(logits))
+            call("g4_softcap_argmax", h, _ptr(logits), rows, cfg.vocab, C.c_float(cfg.softcap), _ptr(ids), _ptr(vals))
+
+    def prefill(self, seq: int, ids, sampling: Sampling | None = None) -> int:
         """greedy(tokenIds, startPos) for one sequence: appends the tokens at its current
-        position and returns the next token id."""
+        position and returns the next token id (sampled by row 0 of `sampling`, if given)."""
         ids = np.asarray(ids, dtype=np.int32)
         T = int(ids.size)
         if T < 1 or T > self.max_rows:
@@ -454,7 +498,7 @@ class Gemma4Model:
             raise G4Error(-6, f"KV cache capacity {self.max_seq} exceeded")
         self.buf["ids"][:T].copy_(torch.from_numpy(ids))
         rmap = G4Rows(self.seq_pos.data_ptr() + 0, seq, T, 0)
-        self._forward(self.buf["ids"], T, rmap, 1, T - 1)
+        self._forward(self.buf["ids"], T, rmap, 1, T - 1, sampling)
         call("g4_advance_positions", self.ctx.handle, _ptr(self.seq_pos), seq, 1, T)
         self.ctx.check_device()
         return int(self.buf["next"][0].item())
@@ -473,14 +517,16 @@ class Gemma4Model:
                 self._dec = False
         return self._dec or None
 
-    def decode_step(self, ids_dev: torch.Tensor | None = None, batch: int | None = None) -> torch.Tensor:
-        """One greedy decode step of sequences 0..batch-1 (row b = sequence b); reads the
-        current tokens from ids_dev (default: the previous step's picks) and returns the
-        device tensor of the next tokens."""
+    def decode_step(self, ids_dev: torch.Tensor | None = None, batch: int | None = None,
+                    sampling: Sampling | None = None) -> torch.Tensor:
+        """One decode step of sequences 0..batch-1 (row b = sequence b), greedy or sampled;
+        reads the current tokens from ids_dev (default: the previous step's picks) and returns
+        the device tensor of the next tokens (buf["val"]: their capped logits, or their
+        probabilities when sampled)."""
         B = batch or self.max_batch
         if ids_dev is not None:
             self.buf["next"][:B].copy_(ids_dev[:B])
-        dec = self.decoder() if B == 1 else None
+        dec = self.decoder() if B == 1 and sampling is None else None
         if dec is not None:  # the whole step in one launch: reads next[0], writes next[0] and val[0]
             dec.step(self.ctx, self.buf["next"], self.seq_pos, self.buf["next"], self.buf["val"])
             return self.buf["next"][:1]
@@ -489,15 +535,71 @@ class Gemma4Model:
         # launches of the graph, so the attention may stream them before its wait.
         flags = _lib.G4_ROWS_HISTORY_READY if self._capturing else 0
         rmap = G4Rows(self.seq_pos.data_ptr(), 0, 1, 0, flags)
-        self._forward(self.buf["ids"], B, rmap, B, 0)
+        self._forward(self.buf["ids"], B, rmap, B, 0, sampling)
         call("g4_advance_positions", self.ctx.handle, _ptr(self.seq_pos), 0, B, 1)
         return self.buf["next"][:B]
 
-    def capture_decode(self, batch: int | None = None):
-        """Captures one decode step (next <- argmax(model(next))) in a CUDA graph."""
+    # --------------------------------------------- drafted trees and forks ---
+    def _own_caches(self) -> list[KVCache]:
+        return [Ly["kv"] for Ly in self.layers if not Ly["spec"]["shared"]]
+
+    def verify_step(self, tokens: torch.Tensor, parents: torch.Tensor, counts: torch.Tensor | None = None,
+                    sampling: Sampling | None = None) -> dict:
+        """One step of drafted decoding of sequences 0..B-1: tokens int32 [B, n] holds a tree of
+        drafted tokens per sequence, node 0 the sequence's current token (the last pick, not yet
+        in the cache), parents int32 [B, n] or [n] the trees (g4_tree).  One forward runs every
+        node, the model's pick after each node is taken (greedy, or sampled by row b * n + i of
+        `sampling`), the path whose drafted tokens equal those picks is accepted, its K/V rows are
+        moved together and the positions advanced by its length.  Returns device tensors: picks
+        [B, n], path [B, n] (-1 behind it), accepted [B] and next [B] (also in buf["next"]), the
+        pick after the path.  Greedy picks give the tokens of as many decode steps; sampled ones
+        their distribution, since each accepted token is the sample drawn at its node."""
+        B, n = tokens.shape
+        rows = B * n
+        if B > self.max_batch or rows > self.max_rows:
+            raise G4Error(-1, f"verify_step: {B} trees of {n} nodes (max_batch {self.max_batch}, max_rows {self.max_rows})")
+        if tokens.dtype != torch.int32 or not tokens.is_contiguous() or tokens.device != self.dev:
+            raise G4Error(-1, f"verify_step: tokens must be a contiguous int32 tensor on {self.dev}")
+        tree = self.ops._tree("verify_step", parents, B, n, counts)
+        picks = self._tree_buffer("picks", rows, torch.int32)
+        if counts is not None:  # unused nodes: any valid token, their rows are not looked at
+            self.buf["ids"][:rows].copy_(tokens.reshape(-1).clamp(0, self.cfg.vocab - 1))
+        else:
+            self.buf["ids"][:rows].copy_(tokens.reshape(-1))
+        flags = _lib.G4_ROWS_HISTORY_READY if self._capturing else 0
+        rmap = G4Rows(self.seq_pos.data_ptr(), 0, n, 0, flags)
+        self._layers(self.buf["ids"], rows, rmap, tree)
+        logits = self._tree_buffer("logits", rows * self.cfg.vocab, torch.float32) if sampling is not None or rows <= 16 else None
+        self._pick(self.buf["x"], rows, picks, self._tree_buffer("vals", rows, torch.float32), logits, sampling)
+        picks = picks[:rows].view(B, n)
+        path, accepted, nxt = self.ops.treeAccept(parents, tokens, picks, counts)
+        kv_compact(self.ctx, self._own_caches(), self.seq_pos, path, accepted, seq_stride=self.max_seq)
+        call("g4_advance_positions_each", self.ctx.handle, _ptr(self.seq_pos), 0, B, _ptr(accepted))
+        self.buf["next"][:B].copy_(nxt if counts is None else torch.where(accepted > 0, nxt, self.buf["next"][:B]))
+        return {"picks": picks, "path": path, "accepted": accepted, "next": self.buf["next"][:B]}
+
+    def _tree_buffer(self, name: str, n: int, dtype) -> torch.Tensor:
+        t = self.buf.get("tree_" + name)
+        if t is None or t.numel() < n:
+            t = self.buf["tree_" + name] = torch.zeros(n, dtype=dtype, device=self.dev)
+        return t
+
+    def fork(self, src: int, dst) -> None:
+        """Copies sequence src (its cached rows, position and last pick) to the sequences dst:
+        several completions of one prompt."""
+        dst = [int(d) for d in dst]
+        if not all(0 <= d < self.max_batch for d in (*dst, src)):
+            raise G4Error(-6, f"fork: sequences {src} -> {dst} of {self.max_batch}")
+        kv_fork(self.ctx, self._own_caches(), self.seq_pos, [src] * len(dst), dst, seq_stride=self.max_seq)
+        if dst:
+            self.buf["next"][torch.tensor(dst, device=self.dev)] = self.buf["next"][src].clone()
+
+    def capture_decode(self, batch: int | None = None, sampling: Sampling | None = None):
+        """Captures one decode step (next <- argmax(model(next)), or the sampled pick with the
+        numbers that sampling.uniform holds at each replay) in a CUDA graph."""
         B = batch or self.max_batch
         saved = self.buf["next"][:B].clone()
-        self.decode_step(batch=B)  # warm-up: sizes workspaces and sets kernel attributes
+        self.decode_step(batch=B, sampling=sampling)  # warm-up: sizes workspaces and sets kernel attributes
         self.ctx.sync()
         self.seq_pos[:B] -= 1      # undo the warm-up step (its K/V slot is rewritten by the replay)
         self.buf["next"][:B].copy_(saved)
@@ -511,7 +613,7 @@ class Gemma4Model:
             self._capturing = True
             try:
                 with torch.cuda.graph(g, stream=stream):
-                    self.decode_step(batch=B)
+                    self.decode_step(batch=B, sampling=sampling)
             finally:
                 self._capturing = False
         self.ctx.set_stream(old)
