@@ -191,5 +191,13 @@ def check(status: int) -> None:
         raise G4Error(status, msg or STATUS_NAMES.get(status, str(status)))
 
 
+_entry = {}  # entry points by name, as ctypes resolved them
+
+
 def call(name: str, *args) -> None:
-    check(getattr(load(), name)(*args))
+    fn = _entry.get(name)
+    if fn is None:
+        fn = _entry[name] = getattr(load(), name)
+    status = fn(*args)
+    if status != G4_OK:
+        check(status)

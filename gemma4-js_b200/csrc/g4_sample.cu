@@ -1071,6 +1071,10 @@ struct General {
             double all;
             const double before = above + block_prefix(x, S.scratch, flip, &all);
             const double past = block_prefix((double)n, S.scratch, flip, &all);  // logits in the parts above
+            if (count && step == 0 && all <= t) {  // no more than are asked for
+                *ok = true;
+                return lim;
+            }
             if (q >= 0 && before < t && before + x >= t) atomicMax(&S.at, q);
             __syncthreads();
             const int at = max(S.at, 0);
@@ -1422,9 +1426,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_general_kernel(const Sampl
         auto prefix = [&](double t, bool count) {
             bool ok;
             const Limit e = g.estimate(lim, t, count, &ok);
-            return ok ? e : g.search(lim, t, count);
+            if (ok) return e;
+            return count && g.number(lim) <= t ? lim : g.search(lim, t, count);
         };
-        if (st.k && g.number(lim) > st.k) lim = prefix((double)st.k, true);
+        if (st.k) lim = prefix((double)st.k, true);
         if (st.p < 1.0) {
             double total = 0.0;
             if (st.k) {
@@ -1466,9 +1471,12 @@ extern "C" g4_status g4_sample(g4_ctx* ctx, const float* logits, long long ld, i
     const int vec = reinterpret_cast<uintptr_t>(logits) % 16 == 0 && (ld % 4 == 0 || rows == 1);
     const int vec4 = vec && vocab % 4 == 0;  // every row in whole 16-byte pieces
 
-    // The general kernel's cluster: parts of at most 16384 logits if 16 CTAs are enough for that.
+    // The general kernel's cluster: parts of at most 16384 logits if 16 CTAs are enough for that, and
+    // down to 4096 while two CTAs per SM hold a cluster for every row.
     int ranks = 1;
-    while (ranks < kMaxCluster && (vocab + ranks - 1) / ranks > 2 * kThreads * 4) ranks <<= 1;
+    while (ranks < kMaxCluster && ((vocab + ranks - 1) / ranks > 8 * kThreads * 4 ||
+                                   ((vocab + ranks - 1) / ranks > 2 * kThreads * 4 && 2LL * ranks * rows <= 2 * ctx->num_sms)))
+        ranks <<= 1;
     const int J = (vocab + ranks * kThreads * 4 - 1) / (ranks * kThreads * 4);
     const size_t gsmem = ((sizeof(GeneralShared) + 15) & ~size_t(15)) + (size_t)J * kThreads * 4 * sizeof(float);
     static_assert(24 * kThreads * 16 + sizeof(GeneralShared) + 16 <= 227 * 1024, "the longest row's parts fit");
@@ -1499,7 +1507,7 @@ extern "C" g4_status g4_sample(g4_ctx* ctx, const float* logits, long long ld, i
                     vec4);
     // Only top-k, top-p and min-p can leave a row to the general kernel.
     if (!st && (how->top_k || how->top_p || how->min_p)) {
-        const int clusters = std::max(1, std::min(rows, 288 / ranks));
+        const int clusters = std::max(1, std::min(rows, 2 * ctx->num_sms / ranks));
         st = g4::launch(ctx, "sample_general_kernel", sample_general_kernel, dim3(clusters * ranks), dim3(kThreads), gsmem,
                         ranks, P, J, vec4);
     }
