@@ -9,6 +9,14 @@
 // are written twice, the second copy in rows ring..ring+mirror-1, so that a key tile of up
 // to `mirror` rows that starts at any slot reads contiguous rows (one TMA box, no split
 // at the wrap).  mirror = 16384 / hd, the widest key tile of the attention kernels.
+// Drafted-tree attention: tensor maps [64 columns][rows][hd / 64] with boxes that fill a whole
+// granule of its ring in one copy (g4_tree_attention.cu); a ring cache's boxes have at most `mirror`
+// rows.
+struct g4_tree_maps {
+    CUtensorMap k, v;
+    int krows = 0, vrows = 0;   // rows of their boxes
+};
+
 struct g4_kv {
     g4_ctx* ctx = nullptr;
     int device = 0;             // of ctx, which may be destroyed before the cache
@@ -22,10 +30,7 @@ struct g4_kv {
     uint16_t* v = nullptr;
     CUtensorMap kmap, vmap;     // 128B-swizzled boxes of 64 columns x (16384/hd) rows
     CUtensorMap kmap_narrow, vmap_narrow;  // the same with boxes of (8192/hd) rows
-    // Drafted-tree attention: [64 columns][rows][hd / 64] with boxes that fill a whole granule of
-    // its ring in one copy (g4_tree_attention.cu); a ring cache's boxes have at most `mirror` rows.
-    CUtensorMap tree_kmap, tree_vmap;
-    int tree_krows = 0, tree_vrows = 0;  // rows of their boxes
+    g4_tree_maps tree[2];       // drafted-tree attention: single CTAs, pairs
 };
 
 namespace g4 {

@@ -37,20 +37,31 @@ constexpr int kThreads = kSoftmaxThreads + 64;  // + TMA warp + MMA warp
 // apart); a V granule holds every column of kVKeys keys (MN-major operand: 64-column chunks
 // kVKeys * 128 B apart, 8-key groups 1024 B apart).  hd 512: a CTA computes all scores but only
 // 256 columns of O, because O (f32) and the two score buffers share 512 TMEM columns.
-template <int HD>
+//
+// kPair: two CTAs of a cluster take 256 rows together (tcgen05 cta_group::2).  Each holds its own
+// rows of Q, S, P and O, but half of K's keys and half of V's columns, which the tensor cores of
+// both read: half the L2 and shared-memory traffic per row.  The even CTA issues every product;
+// commits arrive in both, and the odd one's MMA warp tells it when a granule has landed there.
+// Taken where a sequence has more than 128 rows: one sequence over a long cache at hd 512, whose
+// CTAs read K for 256 columns of V only, 83.7 us in single CTAs, 65.8 in pairs; hd 256, 61.7 and 60.6.
+template <int HD, bool kPair>
 struct TreeCfg {
     static constexpr int HDV = HD < 256 ? HD : 256;           // O columns per CTA
-    static constexpr int NV = HD / HDV;                        // CTAs per 128 rows
+    static constexpr int NV = HD / HDV;                        // CTAs (pairs) per 128 (256) rows
     static constexpr int QBYTES = HD * 256;
-    static constexpr int SLOT = HD == 64 ? 16384 : 32768;
-    static constexpr int KGRAN = HD * 256 / SLOT;              // granules per K tile
-    static constexpr int KBOXES = SLOT / 16384;                // boxes per K granule
-    static constexpr int VGRAN = HDV * 256 / SLOT;
+    static constexpr int KKEYS = kPair ? kTile / 2 : kTile;    // of a tile's keys in this CTA's K
+    static constexpr int VCOLS = kPair ? HDV / 2 : HDV;        // columns of this CTA's V
+    static constexpr int SLOT = HD == (kPair ? 128 : 64) ? 16384 : 32768;
+    static constexpr int KGRAN = HD * KKEYS * 2 / SLOT;        // granules per K tile
+    static constexpr int KBOX = KKEYS * 128;                   // bytes of a K box
+    static constexpr int KBOXES = SLOT / KBOX;                 // boxes per K granule
+    static constexpr int VGRAN = VCOLS * 256 / SLOT;
     static constexpr int VKEYS = kTile / VGRAN;                // keys per V granule
     static constexpr int VBOX = VKEYS * 128;                   // bytes of a V box
-    static constexpr int SLOTS = HD == 64 ? 8 : (229376 - QBYTES) / SLOT;
-    static constexpr int SMEM = QBYTES + SLOTS * SLOT + 3072;  // the rest: alignment (1008), TreeShared
+    static constexpr int SLOTS = SLOT == 16384 ? 8 : (229376 - QBYTES) / SLOT;
+    static constexpr int SMEM = QBYTES + SLOTS * SLOT + 3072;  // the rest: TreeShared
     static_assert(SMEM <= 232448, "shared memory");
+    static_assert(!kPair || HD >= 128, "half of V is whole 64-column chunks");
 };
 
 struct TreeAttnParams {
@@ -67,12 +78,15 @@ struct TreeAttnParams {
 
 struct TreeShared {
     uint64_t full[8], empty[8];
-    uint64_t q_full, s_full[2], p_ready[2], o_done[2], v_full, drained;
+    uint64_t peer_full[8];  // pairs: the granule has landed in the odd CTA
+    uint64_t q_full, s_full[2], p_ready[2], o_done[2], v_full, scanned, drained;
     uint32_t tmem;
     uint32_t poison[3][4];  // keys of a masked tile whose V row is not finite (three tiles in turn)
     int parents[G4_TREE_MAX_NODES];
     float mx[2][2][kRowsPerCta];  // a row's maximum of each half (two tiles in turn); at the end its sums
 };
+
+static_assert(sizeof(TreeShared) <= 3072, "shared memory");
 
 __device__ __forceinline__ float ex2(float x) {  // 2^x to 2^-22, 0 for -inf
     float y;
@@ -86,19 +100,117 @@ __device__ __forceinline__ float ex2(float x) {  // 2^x to 2^-22, 0 for -inf
 // `chunk`: for an MN-major operand, the distance of its 64-element chunks in bytes.
 constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
 __device__ __forceinline__ uint32_t desc_lo(uint32_t saddr, uint32_t chunk = 16) { return saddr >> 4 | (chunk >> 4) << 16; }
+template <bool kPair>
 __device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
-        "mov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}" ::"r"(d),
-        "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(kDescHi));
+    if constexpr (kPair)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
+            "mov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\tsetp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::f16 [%0], a, b, %3, p;\n\t}" ::"r"(d),
+            "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(kDescHi));
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
+            "mov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\tsetp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}" ::"r"(d),
+            "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(kDescHi));
 }
+template <bool kPair>
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a_tmem, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\t"
-        "mov.b64 b, {%2, %5};\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}" ::"r"(d),
-        "r"(a_tmem), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(kDescHi));
+    if constexpr (kPair)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\t"
+            "mov.b64 b, {%2, %5};\n\tsetp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], b, %3, p;\n\t}" ::"r"(d),
+            "r"(a_tmem), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(kDescHi));
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\t"
+            "mov.b64 b, {%2, %5};\n\tsetp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}" ::"r"(d),
+            "r"(a_tmem), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(kDescHi));
+}
+// Arrives on `bar` (in both CTAs of a pair) when the products issued so far have completed.
+template <bool kPair>
+__device__ __forceinline__ void commit_to(uint64_t* bar) {
+    if constexpr (kPair)
+        asm volatile(
+            "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+                smem_u32(bar)),
+            "h"((uint16_t)3)
+            : "memory");
+    else
+        tc_commit(bar);
+}
+template <bool kPair>
+__device__ __forceinline__ void tree_tmem_alloc(uint32_t* dst) {
+    if constexpr (kPair) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(dst)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+    } else {
+        tmem_alloc(dst, 512);
+    }
+}
+template <bool kPair>
+__device__ __forceinline__ void tree_tmem_dealloc(uint32_t tmem) {
+    if constexpr (kPair)
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+    else
+        tmem_dealloc(tmem, 512);
+}
+// Every thread of the pair (of the CTA).
+template <bool kPair>
+__device__ __forceinline__ void pair_sync() {
+    if constexpr (kPair)
+        asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+    else
+        __syncthreads();
+}
+// The address of a shared-memory object in CTA `rank` of the pair.
+__device__ __forceinline__ uint32_t in_cta(const void* p, int rank) {
+    uint32_t a;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+    return a;
+}
+// Arrives on a barrier of either CTA.  kRemote: stores to the other CTA's shared memory come before
+// it; that release at cluster scope costs 1300 to 4000 clocks.  Without any, what comes before is
+// local and complete: a copy that the thread has seen land, tensor-memory stores (tcgen05.wait::st
+// and tcgen05.fence) or stores to its own shared memory behind a proxy fence, which the products
+// read there.
+template <bool kRemote>
+__device__ __forceinline__ void arrive_in(uint64_t* bar, int rank) {
+    if constexpr (kRemote)
+        asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(in_cta(bar, rank)) : "memory");
+    else
+        asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(in_cta(bar, rank)) : "memory");
+}
+__device__ __forceinline__ void or_in(uint32_t* word, int rank, uint32_t bits) {
+    asm volatile("red.relaxed.cluster.shared::cluster.or.b32 [%0], %1;" ::"r"(in_cta(word, rank)), "r"(bits) : "memory");
+}
+// A warp's wait.  kRemote: the other CTA arrives on the barrier.
+template <bool kRemote>
+__device__ __forceinline__ bool wait_on(uint64_t* bar, uint32_t parity, uint32_t* err, uint32_t site) {
+    if constexpr (!kRemote) return mbar_wait_warp(bar, parity, err, site);
+    bool ok = true;
+    unsigned long long t0 = 0;
+    for (;;) {
+        uint32_t done;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(done)
+            : "r"(smem_u32(bar)), "r"(parity), "r"(kPollSuspendNs)
+            : "memory");
+        if (done) break;
+        if (t0 == 0) t0 = globaltimer_ns();
+        else if (globaltimer_ns() - t0 > kWaitLimitNs) {
+            raise_error(err, G4_DEVERR_TIMEOUT, site);
+            ok = false;
+            break;
+        }
+    }
+    return __all_sync(0xffffffffu, ok);
 }
 __device__ __forceinline__ bool elect_one() {
     uint32_t e;
@@ -133,18 +245,22 @@ __device__ __forceinline__ bool tree_seq_fits(const TreeAttnParams& p, const Tre
     return t.base >= 0 && (long long)t.base + count <= p.limit;
 }
 
-template <int HD>
+template <int HD, bool kPair>
 __global__ void __launch_bounds__(kThreads, 1)
 tree_attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                       const TreeAttnParams p) {
-    using C = TreeCfg<HD>;
-    extern __shared__ __align__(1024) uint8_t smem_raw[];
-    uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    using C = TreeCfg<HD, kPair>;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    if (smem_u32(smem) & 1023u) {  // the swizzle needs it, and nothing is left to move the base (never seen)
+        raise_error(p.err, G4_DEVERR_TIMEOUT, 716);
+        return;
+    }
     uint8_t* qsm = smem;
     uint8_t* ring = smem + C::QBYTES;
     TreeShared& sh = *reinterpret_cast<TreeShared*>(ring + C::SLOTS * C::SLOT);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int mtile = blockIdx.x / C::NV, vhalf = blockIdx.x % C::NV;
+    const int rank = kPair ? blockIdx.x & 1 : 0, unit = kPair ? blockIdx.x >> 1 : blockIdx.x;
+    const int vhalf = unit % C::NV, mtile = kPair ? unit / C::NV * 2 + rank : unit / C::NV;
     const int s = blockIdx.y, split = blockIdx.z;
     const int n = p.tree.nodes;
 
@@ -167,7 +283,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
             const bool in = f0 + qr < n * p.heads;
             asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
                              smem_u32(qsm + (c >> 3) * 16384 + qr * 128 + (((c & 7) ^ (qr & 7)) << 4))),
-                         "l"(qg + (in ? u : 0)), "r"(in ? 16 : 0)
+                         "l"(in ? qg + u : reinterpret_cast<const uint4*>(p.q)), "r"(in ? 16 : 0)
                          : "memory");
         }
         if (threadIdx.x < n) parent = p.tree.parents[(size_t)s * p.tree.parent_stride + threadIdx.x];
@@ -178,29 +294,32 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
         for (int i = 0; i < C::SLOTS; ++i) {
             mbar_init(&sh.full[i], 1);
             mbar_init(&sh.empty[i], 1);
+            mbar_init(&sh.peer_full[i], 1);
         }
-        mbar_init(&sh.q_full, kSoftmaxThreads);
+        constexpr int kArrivals = kSoftmaxWarps * (kPair ? 2 : 1);  // a warp each
+        mbar_init(&sh.q_full, kArrivals);
         for (int i = 0; i < 2; ++i) {
             mbar_init(&sh.s_full[i], 1);
-            mbar_init(&sh.p_ready[i], kSoftmaxThreads);
+            mbar_init(&sh.p_ready[i], kArrivals);
             mbar_init(&sh.o_done[i], 1);
         }
         mbar_init(&sh.v_full, 1);
+        mbar_init(&sh.scanned, kArrivals);
         mbar_init(&sh.drained, 1);
         fence_mbar_init();
     }
-    if (warp == kSoftmaxWarps + 1) tmem_alloc(&sh.tmem, 512);
+    if (warp == kSoftmaxWarps + 1) tree_tmem_alloc<kPair>(&sh.tmem);
     // This split's tiles; tile t covers keys lo + (t0 + t) * 128 ...
     const int t0 = (int)((unsigned)split * (unsigned)ts.ntiles / (unsigned)p.nsplit);
     int nt = (int)((unsigned)(split + 1) * (unsigned)ts.ntiles / (unsigned)p.nsplit) - t0;
     const int key0 = ts.lo + t0 * kTile;
     if (ts.base < 0 || ts.base > p.limit) nt = 0;
-    if (!p.history_ready) {  // no used row among this CTA's
+    if (!p.history_ready) {  // no used row among this CTA's (this pair's)
         const int c = tree_count(p.tree, s, nullptr);
-        if (mtile * kRowsPerCta >= c * p.heads || !tree_seq_fits(p, ts, c)) nt = 0;
+        if ((mtile - rank) * kRowsPerCta >= c * p.heads || !tree_seq_fits(p, ts, c)) nt = 0;
     }
     tc_fence_before();
-    __syncthreads();
+    pair_sync<kPair>();
     tc_fence_after();
     const uint32_t tmem = sh.tmem;
     const uint32_t o_tmem = tmem + 256;
@@ -253,7 +372,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
                     for (int a = 0; a < C::KGRAN && ok; ++a, ++g) {
                         const int slot = claim();
                         if (!ok) break;
-                        load(&kmap, slot, a * C::KBOXES, C::KBOXES, k0, kTile, p.krows);
+                        load(&kmap, slot, a * C::KBOXES, C::KBOXES, k0 + rank * C::KKEYS, C::KKEYS, p.krows);
                     }
                 }
                 if (t >= 0) {
@@ -261,7 +380,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
                     for (int a = 0; a < C::VGRAN && ok; ++a, ++g) {
                         const int slot = claim();
                         if (!ok) break;
-                        load(&vmap, slot, vhalf * 4, C::HDV / 64, k0 + a * C::VKEYS, C::VKEYS, p.vrows);
+                        load(&vmap, slot, vhalf * 4 + rank * (C::VCOLS / 64), C::VCOLS / 64, k0 + a * C::VKEYS, C::VKEYS, p.vrows);
                     }
                 }
             }
@@ -272,31 +391,55 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
     } else if (warp == kSoftmaxWarps + 1) {
         // --------------------------------------------------- MMA issuer --
         // The warp stays together (its waits and addresses are uniform); one lane issues.
-        if (nt > 0) {
-            constexpr uint32_t qk_idesc = mma_idesc_bf16(128, kTile);
-            constexpr uint32_t pv_idesc = mma_idesc_bf16(128, C::HDV) | kTransposeB;
+        int slot = 0;
+        uint32_t phase = 0;  // of the slot that comes next in ring order
+        auto next = [&]() {
+            if (++slot == C::SLOTS) slot = 0, phase ^= 1;
+        };
+        if (kPair && rank == 1) {
+            // Only tells the even CTA (and, of a masked tile's V, the softmax threads) what has landed here.
+            bool ok = true;
+            int handed = 0;
+            for (int t = -1; t < nt && ok && nt > 0; ++t) {
+                for (int a = 0; a < (t + 1 < nt ? C::KGRAN : 0) + (t >= 0 ? C::VGRAN : 0) && ok; ++a) {
+                    ok = wait_on<false>(&sh.full[slot], phase, p.err, 714);
+                    if (ok && lane == 0) arrive_in<false>(&sh.peer_full[slot], 0);
+                    __syncwarp();
+                    next();
+                }
+                if (ok && t >= 0 && masked_tile(t)) {
+                    // One hand-over at a time: this warp follows the copies, which may be tiles ahead.
+                    if (handed > 0) ok = wait_on<true>(&sh.scanned, (handed - 1) & 1, p.err, 717);
+                    if (ok && lane == 0) mbar_arrive(&sh.v_full);
+                    ++handed;
+                }
+                __syncwarp();
+            }
+        } else if (nt > 0) {
+            constexpr int kM = kPair ? 256 : 128;
+            constexpr uint32_t qk_idesc = mma_idesc_bf16(kM, kTile);
+            constexpr uint32_t pv_idesc = mma_idesc_bf16(kM, C::HDV) | kTransposeB;
             const uint32_t qa = desc_lo(smem_u32(qsm)), ka = desc_lo(smem_u32(ring));
             const uint32_t va = desc_lo(smem_u32(ring), C::VBOX);
-            bool ok = mbar_wait_warp(&sh.q_full, 0, p.err, 703);
-            int slot = 0;
-            uint32_t phase = 0;  // of the slot that comes next in ring order
-            auto next = [&]() {
-                if (++slot == C::SLOTS) slot = 0, phase ^= 1;
+            bool ok = wait_on<kPair>(&sh.q_full, 0, p.err, 703);
+            auto landed = [&](int sl, uint32_t ph) {
+                ok = ok && wait_on<false>(&sh.full[sl], ph, p.err, 704);
+                if (kPair) ok = ok && wait_on<true>(&sh.peer_full[sl], ph, p.err, 705);
+                return ok;
             };
             auto scores = [&](int t) {
 #pragma unroll
                 for (int a = 0; a < C::KGRAN; ++a) {
-                    ok = ok && mbar_wait_warp(&sh.full[slot], phase, p.err, 704);
-                    if (!ok) return;
+                    if (!landed(slot, phase)) return;
                     tc_fence_after();
                     if (elect_one()) {
                         const uint32_t b = ka + slot * (C::SLOT >> 4), d = tmem + (t & 1) * 128;
 #pragma unroll
                         for (int i = 0; i < C::KBOXES * 4; ++i)
-                            mma_ss(d, qa + (((a * C::KBOXES + i / 4) * 16384 + (i % 4) * 32) >> 4),
-                                   b + (((i / 4) * 16384 + (i % 4) * 32) >> 4), qk_idesc, (a | i) ? 1u : 0u);
-                        tc_commit(&sh.empty[slot]);
-                        if (a == C::KGRAN - 1) tc_commit(&sh.s_full[t & 1]);
+                            mma_ss<kPair>(d, qa + (((a * C::KBOXES + i / 4) * 16384 + (i % 4) * 32) >> 4),
+                                          b + (((i / 4) * C::KBOX + (i % 4) * 32) >> 4), qk_idesc, (a | i) ? 1u : 0u);
+                        commit_to<kPair>(&sh.empty[slot]);
+                        if (a == C::KGRAN - 1) commit_to<kPair>(&sh.s_full[t & 1]);
                     }
                     __syncwarp();
                     next();
@@ -309,35 +452,34 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
                     int sl = slot;
                     uint32_t ph = phase;
                     for (int a = 0; a < C::VGRAN && ok; ++a) {
-                        ok = mbar_wait_warp(&sh.full[sl], ph, p.err, 708);
+                        ok = wait_on<false>(&sh.full[sl], ph, p.err, 708);
                         if (++sl == C::SLOTS) sl = 0, ph ^= 1;
                     }
                     if (ok && lane == 0) mbar_arrive(&sh.v_full);
                     __syncwarp();
                 }
-                ok = ok && mbar_wait_warp(&sh.p_ready[t & 1], (t >> 1) & 1, p.err, 705);
+                ok = ok && wait_on<kPair>(&sh.p_ready[t & 1], (t >> 1) & 1, p.err, 706);
 #pragma unroll
                 for (int a = 0; a < C::VGRAN; ++a) {
-                    ok = ok && mbar_wait_warp(&sh.full[slot], phase, p.err, 706);
-                    if (!ok) break;
+                    if (!landed(slot, phase)) break;
                     tc_fence_after();
                     if (elect_one()) {
                         const uint32_t b = va + slot * (C::SLOT >> 4), w = tmem + (t & 1) * 128;
 #pragma unroll
                         for (int i = 0; i < C::VKEYS / 16; ++i)
-                            mma_ts(o_tmem, w + p_col(a * (C::VKEYS / 16) + i), b + i * (2048 >> 4), pv_idesc,
-                                   (a | i) || t > 0 ? 1u : 0u);
-                        tc_commit(&sh.empty[slot]);
-                        if (a == C::VGRAN - 1) tc_commit(&sh.o_done[t & 1]);
+                            mma_ts<kPair>(o_tmem, w + p_col(a * (C::VKEYS / 16) + i), b + i * (2048 >> 4), pv_idesc,
+                                          (a | i) || t > 0 ? 1u : 0u);
+                        commit_to<kPair>(&sh.empty[slot]);
+                        if (a == C::VGRAN - 1) commit_to<kPair>(&sh.o_done[t & 1]);
                     }
                     __syncwarp();
                     next();
                 }
             }
             // Do not free the tensor memory while products may still be running (after a failed wait).
-            if (elect_one()) tc_commit(&sh.drained);
+            if (elect_one()) commit_to<kPair>(&sh.drained);
             __syncwarp();
-            mbar_wait_warp(&sh.drained, 0, p.err, 711);
+            wait_on<false>(&sh.drained, 0, p.err, 711);
         }
     } else {
         // ------------------ softmax: two threads (warps w, w + 4) per query row --
@@ -361,7 +503,14 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
         const int rows = count * p.heads;              // of this sequence
         asm volatile("cp.async.wait_all;" ::: "memory");
         fence_proxy_async_smem();
-        mbar_arrive(&sh.q_full);
+        auto tell = [&](uint64_t* bar) {  // the issuing CTA, once per warp
+            __syncwarp();
+            if (lane == 0) {
+                if (kPair && rank == 1) arrive_in<false>(bar, 0);
+                else mbar_arrive(bar);
+            }
+        };
+        tell(&sh.q_full);
         asm volatile("bar.sync 1, 256;" ::: "memory");  // parents
         const bool live = f < rows;
         const bool warp_live = f - lane < rows;
@@ -389,7 +538,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
         for (int t = 0; t < nt; ++t) {
             const int k0 = key0 + t * kTile;
             const bool masked = masked_tile(t);
-            ok = ok && mbar_wait_warp(&sh.s_full[t & 1], (t >> 1) & 1, p.err, 707);
+            ok = ok && wait_on<false>(&sh.s_full[t & 1], (t >> 1) & 1, p.err, 707);
             tc_fence_after();
             uint32_t vis[2] = {0xffffffffu, 0xffffffffu};
             if (masked) {
@@ -429,7 +578,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
                     l *= factor;
                 }
                 if (t > 0 && __any_sync(0xffffffffu, grow_m)) {
-                    ok = mbar_wait_warp(&sh.o_done[(t - 1) & 1], ((t - 1) >> 1) & 1, p.err, 709);
+                    ok = wait_on<false>(&sh.o_done[(t - 1) & 1], ((t - 1) >> 1) & 1, p.err, 709);
                     tc_fence_after();
 #pragma unroll 1
                     for (int c = 0; c < C::HDV / 2; c += 32) {
@@ -474,28 +623,28 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
                 const int key = threadIdx.x & 127, vrow = key % C::VKEYS, g = v_granule(t) + key / C::VKEYS;
                 uint32_t* poison = sh.poison[nmasked % 3];
                 if (threadIdx.x < 4) sh.poison[(nmasked + 1) % 3][threadIdx.x] = 0u;  // last read two masked tiles ago
-                ok = ok && mbar_wait_warp(&sh.v_full, nmasked & 1, p.err, 712);
-                ok = ok && mbar_wait_warp(&sh.full[g % C::SLOTS], (g / C::SLOTS) & 1, p.err, 713);  // of this phase now
+                ok = ok && wait_on<false>(&sh.v_full, nmasked & 1, p.err, 712);
+                ok = ok && wait_on<false>(&sh.full[g % C::SLOTS], (g / C::SLOTS) & 1, p.err, 713);  // of this phase now
                 ++nmasked;
                 if (ok) {
                     uint8_t* vr = ring + (g % C::SLOTS) * C::SLOT + vrow * 128;
                     const bool outside = k0 + key >= ts.base + count;
                     bool bad = false;
                     auto at = [&](int i) {
-                        const int c = half * (C::HDV / 16) + i;
+                        const int c = half * (C::VCOLS / 16) + i;
                         return reinterpret_cast<uint4*>(vr + (c >> 3) * C::VBOX + (((c & 7) ^ (vrow & 7)) << 4));
                     };
                     // an exponent of all ones carries into the bit above it
                     auto odd = [](uint32_t e) { return ((e & 0x7f807f80u) + 0x00800080u) & 0x80008000u; };
                     uint32_t any = 0u;
 #pragma unroll 8
-                    for (int i = 0; i < C::HDV / 16; ++i) {
+                    for (int i = 0; i < C::VCOLS / 16; ++i) {
                         const uint4 w = *at(i);
                         any |= odd(w.x) | odd(w.y) | odd(w.z) | odd(w.w);
                     }
                     if (outside || any) {
 #pragma unroll 1
-                        for (int i = 0; i < C::HDV / 16; ++i) {
+                        for (int i = 0; i < C::VCOLS / 16; ++i) {
                             const uint4 w = *at(i);
                             auto clean = [&](uint32_t e) {
                                 const uint32_t o = odd(e);
@@ -505,16 +654,28 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
                         }
                         bad = !outside;
                     }
-                    if (bad) atomicOr(&poison[key >> 5], 1u << lane);
+                    if (bad) {
+                        atomicOr(&poison[key >> 5], 1u << lane);
+                        if (kPair) or_in(&poison[key >> 5], rank ^ 1, 1u << lane);  // its rows see the same keys
+                    }
                     fence_proxy_async_smem();
                 }
-                asm volatile("bar.sync 1, 256;" ::: "memory");
+                if (kPair) {
+                    __syncwarp();
+                    if (lane == 0) {
+                        arrive_in<true>(&sh.scanned, 0);
+                        arrive_in<true>(&sh.scanned, 1);
+                    }
+                    ok = wait_on<true>(&sh.scanned, (nmasked - 1) & 1, p.err, 715) && ok;
+                } else {
+                    asm volatile("bar.sync 1, 256;" ::: "memory");
+                }
 #pragma unroll 1
                 for (int w = 0; w < 4; ++w)
                     if (poison[w] & visible(k0, w)) l = __int_as_float(0x7fffffff);  // sees a V row that is not finite
             }
             tc_fence_before();
-            mbar_arrive(&sh.p_ready[t & 1]);
+            tell(&sh.p_ready[t & 1]);
         }
         // ---- O of the row ----
         if (nt > 0) {
@@ -522,7 +683,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
             sh.mx[nt & 1][half][r] = l;
             asm volatile("bar.sync %0, 64;" ::"r"(2 + (warp & 3)) : "memory");
             l += sh.mx[nt & 1][half ^ 1][r];
-            ok = ok && mbar_wait_warp(&sh.o_done[(nt - 1) & 1], ((nt - 1) >> 1) & 1, p.err, 710);
+            ok = ok && wait_on<false>(&sh.o_done[(nt - 1) & 1], ((nt - 1) >> 1) & 1, p.err, 710);
         }
         tc_fence_after();
         // Rows leave through shared memory (Q and the ring have been read for the last time): written
@@ -586,11 +747,12 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
         }
     }
     tc_fence_before();
-    __syncthreads();
+    __syncwarp();
+    pair_sync<kPair>();  // (of a pair: neither leaves while the other may read its shared memory)
     if (warp == kSoftmaxWarps + 1) {
         __syncwarp();
         tc_fence_after();
-        tmem_dealloc(tmem, 512);
+        tree_tmem_dealloc<kPair>(tmem);
     }
 }
 
@@ -600,8 +762,8 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
 // l = 0 and is left out (its O was not written).
 constexpr int kMaxSplits = 160;
 template <int HD>
-__global__ void __launch_bounds__(TreeCfg<HD>::HDV / 2) tree_combine_kernel(const TreeAttnParams p) {
-    using C = TreeCfg<HD>;
+__global__ void __launch_bounds__(TreeCfg<HD, false>::HDV / 2) tree_combine_kernel(const TreeAttnParams p) {
+    using C = TreeCfg<HD, false>;
     constexpr int T = C::HDV / 2;
     __shared__ float2 ml[kMaxSplits];
     pdl_trigger();
@@ -633,21 +795,22 @@ __global__ void __launch_bounds__(TreeCfg<HD>::HDV / 2) tree_combine_kernel(cons
     reinterpret_cast<uint32_t*>(p.out + row * HD + vhalf * C::HDV)[threadIdx.x] = w;
 }
 
-template <int HD>
-g4_status launch_tree_attention(g4_ctx* ctx, const g4_kv* kv, TreeAttnParams p) {
-    using C = TreeCfg<HD>;
+template <int HD, bool kPair>
+g4_status launch_tree_attention_t(g4_ctx* ctx, const g4_kv* kv, TreeAttnParams p) {
+    using C = TreeCfg<HD, kPair>;
     const int mtiles = (p.tree.nodes * p.heads + kRowsPerCta - 1) / kRowsPerCta;
     const int longest = (p.sliding && p.window < p.seq_stride ? p.window : p.seq_stride) + p.tree.nodes;
     const int ntiles = (longest + kTile - 1) / kTile;
-    const long long ctas = (long long)mtiles * C::NV * p.nseq;
+    const int across = (kPair ? (mtiles + 1) / 2 * 2 : mtiles) * C::NV;  // CTAs of a sequence and split
+    const long long ctas = (long long)across * p.nseq;
     // Split the keys while that adds CTAs to SMs without one, at three tiles or more per split: a
     // split costs its CTA's start and drain (about three tiles' time) and the join.  One sequence
     // of 8 nodes over 4096 keys: 15.0 us at two tiles, 15.3 at three, 19.1 at six; 64 sequences
     // with a window of 512 (five tiles): 28.6 us in two splits, 19.9 whole.
-    int nsplit = (int)std::max<long long>(1, std::min<long long>({ctx->num_sms / ctas, ntiles / 3, kMaxSplits}));
+    const int nsplit = (int)std::max<long long>(1, std::min<long long>({ctx->num_sms / ctas, ntiles / 3, kMaxSplits}));
     p.nsplit = nsplit;
+    const size_t nrows = (size_t)p.nseq * p.tree.nodes * p.heads;
     if (nsplit > 1) {
-        const size_t nrows = (size_t)p.nseq * p.tree.nodes * p.heads;
         const size_t ob = nsplit * nrows * HD * sizeof(float);
         g4_status st = g4::ensure_workspace(ctx, ob + (size_t)nsplit * C::NV * nrows * sizeof(float2));
         if (st) return st;
@@ -656,38 +819,55 @@ g4_status launch_tree_attention(g4_ctx* ctx, const g4_kv* kv, TreeAttnParams p) 
     }
     static std::atomic<uint64_t> attr_set{0};
     if (!(attr_set.load() & (1ull << ctx->device))) {
-        G4_CHECK_CUDA(cudaFuncSetAttribute(tree_attention_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+        G4_CHECK_CUDA(cudaFuncSetAttribute(tree_attention_kernel<HD, kPair>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                           C::SMEM));
         attr_set.fetch_or(1ull << ctx->device);
     }
-    p.krows = kv->tree_krows;
-    p.vrows = kv->tree_vrows;
-    g4_status st = g4::launch(ctx, "tree_attention_kernel", tree_attention_kernel<HD>, dim3(mtiles * C::NV, p.nseq, nsplit),
-                              dim3(kThreads), C::SMEM, 1, kv->tree_kmap, kv->tree_vmap, p);
+    const g4_tree_maps& maps = kv->tree[kPair];
+    p.krows = maps.krows;
+    p.vrows = maps.vrows;
+    g4_status st = g4::launch(ctx, "tree_attention_kernel", tree_attention_kernel<HD, kPair>, dim3(across, p.nseq, nsplit),
+                              dim3(kThreads), C::SMEM, kPair ? 2 : 1, maps.k, maps.v, p);
     if (st || nsplit == 1) return st;
-    const size_t nrows = (size_t)p.nseq * p.tree.nodes * p.heads;
     // The join is set up while the attention runs, and waits for it (griddepcontrol).
     const bool pdl = ctx->pdl;
     ctx->pdl = true;
-    st = g4::launch(ctx, "tree_combine_kernel", tree_combine_kernel<HD>,
-                      dim3((unsigned)nrows, C::NV), dim3(C::HDV / 2), 0, 1, p);
+    st = g4::launch(ctx, "tree_combine_kernel", tree_combine_kernel<HD>, dim3((unsigned)nrows, C::NV), dim3(C::HDV / 2), 0, 1,
+                    p);
     ctx->pdl = pdl;
     return st;
 }
-
 template <int HD>
+g4_status launch_tree_attention(g4_ctx* ctx, const g4_kv* kv, const TreeAttnParams& p) {
+    if constexpr (HD >= 128) {
+        if (p.tree.nodes * p.heads > kRowsPerCta) return launch_tree_attention_t<HD, true>(ctx, kv, p);
+    }
+    return launch_tree_attention_t<HD, false>(ctx, kv, p);
+}
+
+template <int HD, bool kPair>
 g4_status tree_maps(g4_kv* kv) {
-    using C = TreeCfg<HD>;
+    using C = TreeCfg<HD, kPair>;
+    g4_tree_maps& m = kv->tree[kPair];
     const int contiguous = kv->ring ? kv->mirror : kTile;
-    kv->tree_krows = std::min(kTile, contiguous);
-    kv->tree_vrows = std::min(C::VKEYS, contiguous);
+    m.krows = std::min(C::KKEYS, contiguous);
+    m.vrows = std::min(C::VKEYS, contiguous);
     const uint64_t dims[3] = {64, (uint64_t)kv->rows_total, HD / 64}, pitch[2] = {HD * 2, 128};
-    const uint32_t kbox[3] = {64, (uint32_t)kv->tree_krows, kv->tree_krows == kTile ? (uint32_t)C::KBOXES : 1u};
-    const uint32_t vbox[3] = {64, (uint32_t)kv->tree_vrows, kv->tree_vrows == C::VKEYS ? C::HDV / 64u : 1u};
-    g4_status st = g4::encode_tensor_map_3d(&kv->tree_kmap, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, kv->k, dims, pitch, kbox,
+    const uint32_t kbox[3] = {64, (uint32_t)m.krows, m.krows == C::KKEYS ? (uint32_t)C::KBOXES : 1u};
+    const uint32_t vbox[3] = {64, (uint32_t)m.vrows, m.vrows == C::VKEYS ? C::VCOLS / 64u : 1u};
+    g4_status st = g4::encode_tensor_map_3d(&m.k, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, kv->k, dims, pitch, kbox,
                                             CU_TENSOR_MAP_SWIZZLE_128B);
     if (st) return st;
-    return g4::encode_tensor_map_3d(&kv->tree_vmap, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, kv->v, dims, pitch, vbox,
+    return g4::encode_tensor_map_3d(&m.v, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, kv->v, dims, pitch, vbox,
                                     CU_TENSOR_MAP_SWIZZLE_128B);
+}
+template <int HD>
+g4_status tree_maps_all(g4_kv* kv) {
+    g4_status st = tree_maps<HD, false>(kv);
+    if constexpr (HD >= 128) {
+        if (!st) st = tree_maps<HD, true>(kv);
+    }
+    return st;
 }
 
 }  // namespace
@@ -696,10 +876,10 @@ namespace g4 {
 
 g4_status make_tree_maps(g4_kv* kv) {
     switch (kv->hd) {
-        case 64: return tree_maps<64>(kv);
-        case 128: return tree_maps<128>(kv);
-        case 256: return tree_maps<256>(kv);
-        default: return tree_maps<512>(kv);
+        case 64: return tree_maps_all<64>(kv);
+        case 128: return tree_maps_all<128>(kv);
+        case 256: return tree_maps_all<256>(kv);
+        default: return tree_maps_all<512>(kv);
     }
 }
 
