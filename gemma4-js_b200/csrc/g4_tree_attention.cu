@@ -25,9 +25,13 @@ using namespace g4dev;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kTile = 128;        // keys per tile = MMA N of the scores
 constexpr int kRowsPerCta = 128;  // MMA M
-// Two threads per query row, each with half of a tile's keys and half of O's columns: two warps
-// per scheduler hide each other's latencies (one warp per scheduler: 4500 clocks per tile).
-constexpr int kSoftmaxWarps = 8;
+// Four threads per query row, each with a quarter of a tile's keys (scores are read once and stay in
+// registers) and of O's columns: four warps per scheduler hide each other's latencies.  32 sequences
+// of 512 rows over 4160 keys at hd 256: 59.6 us, with two threads per row (scores read twice) 60.6; one
+// per row, a warp per scheduler, took 4500 clocks per tile instead of 2800.
+constexpr int kParts = 4;
+constexpr int kSoftmaxWarps = 4 * kParts;
+constexpr int kKeysPerThread = kTile / kParts;
 constexpr int kSoftmaxThreads = kSoftmaxWarps * 32;
 constexpr int kThreads = kSoftmaxThreads + 64;  // + TMA warp + MMA warp
 
@@ -47,6 +51,7 @@ constexpr int kThreads = kSoftmaxThreads + 64;  // + TMA warp + MMA warp
 template <int HD, bool kPair>
 struct TreeCfg {
     static constexpr int HDV = HD < 256 ? HD : 256;           // O columns per CTA
+    static constexpr int OCOLS = HDV < 128 ? 32 : HDV / kParts;  // O columns per thread (hd 64: of the first parts)
     static constexpr int NV = HD / HDV;                        // CTAs (pairs) per 128 (256) rows
     static constexpr int QBYTES = HD * 256;
     static constexpr int KKEYS = kPair ? kTile / 2 : kTile;    // of a tile's keys in this CTA's K
@@ -83,7 +88,7 @@ struct TreeShared {
     uint32_t tmem;
     uint32_t poison[3][4];  // keys of a masked tile whose V row is not finite (three tiles in turn)
     int parents[G4_TREE_MAX_NODES];
-    float mx[2][2][kRowsPerCta];  // a row's maximum of each half (two tiles in turn); at the end its sums
+    int mx[3][kRowsPerCta];  // a row's maximum, ordered as integers (three tiles in turn)
 };
 
 static_assert(sizeof(TreeShared) <= 3072, "shared memory");
@@ -218,9 +223,12 @@ __device__ __forceinline__ bool elect_one() {
     return e != 0;
 }
 constexpr uint32_t kTransposeB = 1u << 16;
-// Weights (bf16 pairs) lie over the scores they come from, each half of a tile over its own half:
-// TMEM column of the 16-key step i.
-__device__ __forceinline__ int p_col(int i) { return (i >> 2) * 64 + (i & 3) * 8; }
+// Weights (bf16 pairs) lie over the scores they come from, each thread's over its own: TMEM column
+// of the 16-key step i.
+__device__ __forceinline__ int p_col(int i) { return (i >> 1) * kKeysPerThread + (i & 1) * 8; }
+// Floats (but NaN) in the order of integers, and back.
+__device__ __forceinline__ int ordered(int bits) { return bits < 0 ? bits ^ 0x7fffffff : bits; }
+constexpr int kLowest = (int)0x807fffff;  // ordered(-inf)
 
 // Bits [lo, hi) of the word that covers columns 32 w .. 32 w + 31.
 __device__ __forceinline__ uint32_t range_word(int lo, int hi, int w) {
@@ -482,8 +490,8 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
             wait_on<false>(&sh.drained, 0, p.err, 711);
         }
     } else {
-        // ------------------ softmax: two threads (warps w, w + 4) per query row --
-        const int half = warp >> 2, r = (warp & 3) * 32 + lane;
+        // ------------------ softmax: kParts threads (warps w, w + 4, ...) per query row --
+        const int part = warp >> 2, r = (warp & 3) * 32 + lane;
         const int f = f0 + r;
         if (p.history_ready) {
             pdl_wait();
@@ -511,7 +519,10 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
             }
         };
         tell(&sh.q_full);
-        asm volatile("bar.sync 1, 256;" ::: "memory");  // parents
+        if (part < 2) sh.mx[part][r] = kLowest;
+        auto softmax_sync = [&]() { asm volatile("bar.sync 1, %0;" ::"n"(kSoftmaxThreads) : "memory"); };
+        auto row_sync = [&]() { asm volatile("bar.sync %0, %1;" ::"r"(2 + (warp & 3)), "n"(32 * kParts) : "memory"); };
+        softmax_sync();  // parents
         const bool live = f < rows;
         const bool warp_live = f - lane < rows;
         // The row's visible drafted rows (bit = node) and first visible cached key.
@@ -529,8 +540,9 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
             const unsigned long long bits = sft >= 64 || sft <= -32 ? 0ull : sft >= 0 ? seen >> sft : seen << -sft;
             return live ? range_word(first - k0, d, w) | (uint32_t)bits : 0u;
         };
-        const uint32_t s_tmem = tmem + ((uint32_t)((warp & 3) * 32) << 16) + half * 64;
-        const uint32_t o_half = o_tmem + ((uint32_t)((warp & 3) * 32) << 16) + half * (C::HDV / 2);
+        const uint32_t s_tmem = tmem + ((uint32_t)((warp & 3) * 32) << 16) + part * kKeysPerThread;
+        const uint32_t o_part = o_tmem + ((uint32_t)((warp & 3) * 32) << 16) + part * C::OCOLS;
+        const bool has_o = part * C::OCOLS < C::HDV;
         float m = -INFINITY, mu = 0.f, l = 0.f;
         // A warp whose wait gave up keeps to the barriers of the others and does nothing else.
         bool ok = true;
@@ -540,33 +552,25 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
             const bool masked = masked_tile(t);
             ok = ok && wait_on<false>(&sh.s_full[t & 1], (t >> 1) & 1, p.err, 707);
             tc_fence_after();
-            uint32_t vis[2] = {0xffffffffu, 0xffffffffu};
-            if (masked) {
-                vis[0] = visible(k0, 2 * half);
-                vis[1] = visible(k0, 2 * half + 1);
-            }
-            float tm = -INFINITY;
+            uint32_t x[32];
+            int* const mx = sh.mx[t % 3];
             if (warp_live && ok) {
-#pragma unroll 1
-                for (int c = 0; c < 2; ++c) {
-                    uint32_t x[32];
-                    tmem_ld_32x32b_x32(s_tmem + (t & 1) * 128 + c * 32, x);
-                    tmem_ld_wait(x);
-                    if (masked) {
-                        const uint32_t v = c ? vis[1] : vis[0];
+                tmem_ld_32x32b_x32(s_tmem + (t & 1) * 128, x);
+                tmem_ld_wait(x);
+                if (masked) {
+                    const uint32_t v = visible(k0, part);
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) x[i] = v >> i & 1u ? x[i] : 0xff800000u;
-                    }
-                    float m4[4] = {tm, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) m4[i & 3] = fmaxf(m4[i & 3], __uint_as_float(x[i]));
-                    tm = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+                    for (int i = 0; i < 32; ++i) x[i] = v >> i & 1u ? x[i] : 0xff800000u;
                 }
-                sh.mx[t & 1][half][r] = tm;
+                float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int i = 0; i < 32; ++i) m4[i & 3] = fmaxf(m4[i & 3], __uint_as_float(x[i]));
+                atomicMax(&mx[r], ordered(__float_as_int(fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])))));
             }
-            asm volatile("bar.sync %0, 64;" ::"r"(2 + (warp & 3)) : "memory");
+            row_sync();
             if (warp_live && ok) {
-                tm = fmaxf(tm, sh.mx[t & 1][half ^ 1][r]);
+                const float tm = __int_as_float(ordered(mx[r]));
+                if (part == 0) sh.mx[(t + 2) % 3][r] = kLowest;  // last read before this tile's barrier
                 // The weights are taken against a maximum that may be stale by up to 2^8 (P and the
                 // sums have the range for it), so O is rescaled only when it is exceeded.
                 const bool grow_m = tm > m && !((tm - m) * kLog2e <= 8.f);
@@ -577,47 +581,37 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
                     mu = m * kLog2e;
                     l *= factor;
                 }
-                if (t > 0 && __any_sync(0xffffffffu, grow_m)) {
+                if (t > 0 && has_o && __any_sync(0xffffffffu, grow_m)) {
                     ok = wait_on<false>(&sh.o_done[(t - 1) & 1], ((t - 1) >> 1) & 1, p.err, 709);
                     tc_fence_after();
 #pragma unroll 1
-                    for (int c = 0; c < C::HDV / 2; c += 32) {
+                    for (int c = 0; c < C::OCOLS; c += 32) {
                         uint32_t o[32];
-                        tmem_ld_32x32b_x32(o_half + c, o);
+                        tmem_ld_32x32b_x32(o_part + c, o);
                         tmem_ld_wait(o);
 #pragma unroll
                         for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * factor);
-                        tmem_st_32x32b_x32(o_half + c, o);
+                        tmem_st_32x32b_x32(o_part + c, o);
                     }
                 }
                 // P in bf16 (the product's operand type; at most 1 part in 256 per weight) over the
                 // scores just read; l sums the rounded weights, so they are weights of sum 1.
-#pragma unroll 1
-                for (int c = 0; c < 2; ++c) {
-                    uint32_t x[32], w[16];
-                    tmem_ld_32x32b_x32(s_tmem + (t & 1) * 128 + c * 32, x);
-                    tmem_ld_wait(x);
-                    if (masked) {
-                        const uint32_t v = c ? vis[1] : vis[0];
+                uint32_t w[16];
+                float l0 = 0.f, l1 = 0.f;
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) x[i] = v >> i & 1u ? x[i] : 0xff800000u;
-                    }
-                    float l0 = 0.f, l1 = 0.f;
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const float a = ex2(fmaf(__uint_as_float(x[2 * i]), kLog2e, -mu));
-                        const float b = ex2(fmaf(__uint_as_float(x[2 * i + 1]), kLog2e, -mu));
-                        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[i]) : "f"(b), "f"(a));
-                        l0 += __uint_as_float(w[i] << 16);
-                        l1 += __uint_as_float(w[i] & 0xffff0000u);
-                    }
-                    tmem_st_32x32b_x16(s_tmem + (t & 1) * 128 + c * 16, w);
-                    l += l0 + l1;
+                for (int i = 0; i < 16; ++i) {
+                    const float a = ex2(fmaf(__uint_as_float(x[2 * i]), kLog2e, -mu));
+                    const float b = ex2(fmaf(__uint_as_float(x[2 * i + 1]), kLog2e, -mu));
+                    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[i]) : "f"(b), "f"(a));
+                    l0 += __uint_as_float(w[i] << 16);
+                    l1 += __uint_as_float(w[i] & 0xffff0000u);
                 }
+                tmem_st_32x32b_x16(s_tmem + (t & 1) * 128, w);
+                l += l0 + l1;
                 tmem_st_wait();
             }
             if (masked) {
-                // What no row sees must not reach the product: 0 * NaN.  Thread = key and half of the
+                // What no row sees must not reach the product: 0 * NaN.  Thread = key and a part of the
                 // columns: rows behind base + count become 0; values that are not finite become 0 and
                 // are remembered.
                 const int key = threadIdx.x & 127, vrow = key % C::VKEYS, g = v_granule(t) + key / C::VKEYS;
@@ -631,20 +625,20 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
                     const bool outside = k0 + key >= ts.base + count;
                     bool bad = false;
                     auto at = [&](int i) {
-                        const int c = half * (C::VCOLS / 16) + i;
+                        const int c = part * (C::VCOLS / (8 * kParts)) + i;
                         return reinterpret_cast<uint4*>(vr + (c >> 3) * C::VBOX + (((c & 7) ^ (vrow & 7)) << 4));
                     };
                     // an exponent of all ones carries into the bit above it
                     auto odd = [](uint32_t e) { return ((e & 0x7f807f80u) + 0x00800080u) & 0x80008000u; };
                     uint32_t any = 0u;
 #pragma unroll 8
-                    for (int i = 0; i < C::VCOLS / 16; ++i) {
+                    for (int i = 0; i < C::VCOLS / (8 * kParts); ++i) {
                         const uint4 w = *at(i);
                         any |= odd(w.x) | odd(w.y) | odd(w.z) | odd(w.w);
                     }
                     if (outside || any) {
 #pragma unroll 1
-                        for (int i = 0; i < C::VCOLS / 16; ++i) {
+                        for (int i = 0; i < C::VCOLS / (8 * kParts); ++i) {
                             const uint4 w = *at(i);
                             auto clean = [&](uint32_t e) {
                                 const uint32_t o = odd(e);
@@ -668,7 +662,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
                     }
                     ok = wait_on<true>(&sh.scanned, (nmasked - 1) & 1, p.err, 715) && ok;
                 } else {
-                    asm volatile("bar.sync 1, 256;" ::: "memory");
+                    softmax_sync();
                 }
 #pragma unroll 1
                 for (int w = 0; w < 4; ++w)
@@ -679,14 +673,20 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
         }
         // ---- O of the row ----
         if (nt > 0) {
-            // mx[nt & 1] was last read before the barrier of tile nt - 1
-            sh.mx[nt & 1][half][r] = l;
-            asm volatile("bar.sync %0, 64;" ::"r"(2 + (warp & 3)) : "memory");
-            l += sh.mx[nt & 1][half ^ 1][r];
+            // The last product is done, so Q and the ring have been read for the last time.  (A warp whose
+            // wait gave up writes nothing: copies may be landing yet.)
             ok = ok && wait_on<false>(&sh.o_done[(nt - 1) & 1], ((nt - 1) >> 1) & 1, p.err, 710);
+            float* const sums = reinterpret_cast<float*>(ring + C::SLOTS * C::SLOT) - kParts * kRowsPerCta;  // behind the staged rows
+            static_assert(kRowsPerCta * C::HDV * 4 + kParts * kRowsPerCta * 4 <= C::QBYTES + C::SLOTS * C::SLOT, "staging");
+            if (ok) sums[part * kRowsPerCta + r] = l;
+            row_sync();
+            if (ok) {
+                l = 0.f;
+                for (int i = 0; i < kParts; ++i) l += sums[i * kRowsPerCta + r];
+            }
         }
         tc_fence_after();
-        // Rows leave through shared memory (Q and the ring have been read for the last time): written
+        // Rows leave through shared memory: written
         // by row, 16-byte chunks permuted within 128 B against bank conflicts, read back along the
         // rows, so that global stores are whole lines.  (Stores from the row's own thread touch 32
         // lines each: 5 to 10 thousand clocks per CTA.)
@@ -697,13 +697,13 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
                 constexpr bool whole = decltype(whole_c)::value;
                 constexpr int rowb = C::HDV * (whole ? 2 : 4), chunks = rowb / 16;  // of a staged row
                 uint8_t* const mine = smem + r * rowb;
-                if (ok) {
+                if (ok && has_o) {
 #pragma unroll 1
-                    for (int c = 0; c < C::HDV / 2; c += 32) {
+                    for (int c = 0; c < C::OCOLS; c += 32) {
                         uint32_t o[32];
-                        tmem_ld_32x32b_x32(o_half + c, o);
+                        tmem_ld_32x32b_x32(o_part + c, o);
                         tmem_ld_wait(o);
-                        const int col = half * (C::HDV / 2) + c;
+                        const int col = part * C::OCOLS + c;
 #pragma unroll
                         for (int i = 0; i < (whole ? 4 : 8); ++i) {
                             uint32_t w[4];
@@ -722,16 +722,16 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
                                 make_uint4(w[0], w[1], w[2], w[3]);
                         }
                     }
-                    if (!whole && live && half == 0)
+                    if (!whole && live && part == 0)
                         p.part_ml[(split * C::NV + vhalf) * nrows + grow + f] = make_float2(mu, l);
                 }
-                asm volatile("bar.sync %0, 64;" ::"r"(2 + (warp & 3)) : "memory");
+                row_sync();
                 if (ok) {
-                    const int row0 = (warp & 3) * 32;  // the pair's 32 rows
+                    const int row0 = (warp & 3) * 32;  // the row group
                     uint8_t* const to = (whole ? reinterpret_cast<uint8_t*>(p.out) : reinterpret_cast<uint8_t*>(p.part_o)) +
                                         ((whole ? 0 : split * nrows) + grow + f0) * (HD * (whole ? 2 : 4)) + vhalf * rowb;
 #pragma unroll 8
-                    for (int u = half * 32 + lane; u < 32 * chunks; u += 64) {
+                    for (int u = part * 32 + lane; u < 32 * chunks; u += 32 * kParts) {
                         const int rr = row0 + u / chunks, ch = u % chunks;
                         if (f0 + rr < rows)
                             *reinterpret_cast<uint4*>(to + (size_t)rr * (HD * (whole ? 2 : 4)) + ch * 16) =
@@ -741,7 +741,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
             };
             if (p.nsplit == 1) stage(std::true_type{});
             else stage(std::false_type{});
-        } else if (nt == 0 && p.nsplit > 1 && live && half == 0) {
+        } else if (nt == 0 && p.nsplit > 1 && live && part == 0) {
             const size_t nrows = (size_t)p.nseq * n * p.heads;
             p.part_ml[(split * C::NV + vhalf) * nrows + grow + f] = make_float2(0.f, 0.f);
         }
