@@ -58,6 +58,8 @@ constexpr uint32_t kLowestKey = 0x00800000u;  // of -FLT_MAX
 __device__ __forceinline__ float key_logit(uint32_t k) {
     return __uint_as_float(k ^ (k & 0x80000000u ? 0x80000000u : 0xffffffffu));
 }
+// The key before k, without the one of -0, which no logit has and which compares like +0's.
+__device__ __forceinline__ uint32_t key_before(uint32_t k) { return k == 0x80000000u ? 0x7ffffffeu : k - 1u; }
 
 // A row's settings with what is off made explicit.
 enum Mode { kTopK, kAll, kMinP, kTopP, kGeneral };
@@ -1026,7 +1028,7 @@ struct General {
         *ok = false;
         cluster.sync();  // (a histogram of an earlier call may still be read)
         for (int step = 0; step < 5; ++step) {
-            const float a = key_logit(lo), b = key_logit(hi - 1);
+            const float a = key_logit(lo), b = key_logit(key_before(hi));
             if (!(a > -3.0e38f && b < 3.0e38f && a < b)) return lim;
             const float scale = (float)kBins / (b - a);
             if (!(scale < 3.0e38f && scale > 0.f)) return lim;
@@ -1110,7 +1112,7 @@ struct General {
             const uint32_t nlo = b0 > 0 ? edge(b0) : lo, nhi = b1 < kBins - 1 ? edge(b1 + 1) : hi;
             if (in > (double)kPick && nlo == lo && nhi == hi) return lim;
             lo = nlo, hi = nhi;
-            if (!count) above = mass(lim, key_logit(hi - 1));
+            if (!count) above = mass(lim, key_logit(key_before(hi)));
             if (!(above < t)) return lim;
             if (in <= (double)kPick) return rank_window(lim, lo, hi, above, t, count, ok);
         }
@@ -1127,7 +1129,7 @@ struct General {
         for (int step = 0; inside_n > kPick && hi - lo > 1; ++step) {
             uint32_t cut[kWays];
             float cutv[kWays];
-            const float a = key_logit(lo), b = key_logit(hi - 1);
+            const float a = key_logit(lo), b = key_logit(key_before(hi));
             const bool even = (step & 1) == 0 && a > -3.0e38f && b < 3.0e38f && a < b;
 #pragma unroll
             for (int i = 0; i < kWays; ++i) {
@@ -1184,7 +1186,7 @@ struct General {
         cluster.sync();
         int* cnt = cluster.map_shared_rank(&S.ncand, 0);
         unsigned long long* list = cluster.map_shared_rank(&S.cand[0], 0);
-        const float a = key_logit(lo), b = key_logit(hi - 1);
+        const float a = key_logit(lo), b = key_logit(key_before(hi));
         each([&](int i, const float (&v)[4]) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {

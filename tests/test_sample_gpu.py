@@ -165,6 +165,17 @@ def test_rows_in_hard_orders(ops, order):
         check(ops, l, u, **kw)
 
 
+@pytest.mark.parametrize("V", [16384, 50001])
+def test_borders_on_either_side_of_zero(ops, V):
+    """Logits of few values, zero among them: a search whose bounds meet between -0 and +0 counts the
+    zeros on one side only."""
+    l = np.round(np.random.default_rng(V).standard_normal((12, V)) * 12).astype(np.float32) / 8
+    u = np.linspace(0.03, 0.97, 12).astype(np.float32)
+    check(ops, l, u, p=np.linspace(0.4, 0.99, 12))
+    check(ops, l, u, k=(np.linspace(0.2, 0.95, 12) * V).astype(int))
+    check(ops, l, u, k=(np.linspace(0.95, 0.2, 12) * V).astype(int), p=0.97)
+
+
 def test_strided_and_unaligned_rows(ops):
     l, u = rows(7, 1003, 6)
     big = torch.zeros((7, 2048), device="cuda")
