@@ -6,7 +6,7 @@
 // Sums of up to 786432 weights decide which token a border falls on, so weights and sums are
 // 64-bit (32-bit weights would move a border past a token in one row of some hundred).
 //
-// Three launches:
+// Three launches, and a fourth before the last where a top_p is given without a top_k:
 //   summary  reads the logits once (bound by HBM) and leaves, per group of 4 .. 512 consecutive
 //            logits (at most 2048 groups a row), the highest key and, for rows whose settings
 //            need the mass of the whole row, the group's weight relative to its highest logit.
@@ -15,8 +15,10 @@
 //            (64 of 2048 groups: 32 KB of a 1 MB row) and ranked.  Rows it cannot settle that
 //            way (a nucleus of more than some thousand tokens, top-k above 1024, masses of ties)
 //            go to a queue.
+//   nucleus  a cluster of CTAs reads a queued row with a top-p alone twice: once to find what the
+//            prefix can end on, once for its sum and end.
 //   general  a cluster of CTAs holds a queued row in shared memory and narrows the threshold of
-//            each filter by sums over the row; right for every row, some 20 times the cost.
+//            each filter by sums over the row; right for every row.
 #include <algorithm>
 
 #include <cooperative_groups.h>
@@ -44,7 +46,9 @@ struct SampleParams {
     uint32_t* gkey;   // [rows][groups] highest key of each group
     double* gmass;    // [rows][groups] sum of exp((l - group's highest) / T)
     double* rowmass;  // [rows] weight of the whole row, for rows left to the general kernel with a top_p and no top_k
+    uint32_t* rowkey; // [rows] highest key, for rows left to the nucleus kernel
     int* queue;       // [0] rows left to the general kernel, then the rows
+    int* nucleus;     // the same for the nucleus kernel; null: not launched
     int gshift, groups;
 };
 
@@ -130,7 +134,10 @@ template <bool kVec>
 __global__ void __launch_bounds__(kSumWarps * 32) sample_summary_kernel(const SampleParams P, int segments) {
     pdl_trigger();
     pdl_wait();
-    if (blockIdx.x == 0 && threadIdx.x == 0) P.queue[0] = 0;
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+        P.queue[0] = 0;
+        if (P.nucleus) P.nucleus[0] = 0;
+    }
     const int lane = threadIdx.x & 31;
     const int r = (int)(blockIdx.x / (unsigned)segments);
     const int base = ((int)(blockIdx.x - (unsigned)r * segments) * kSumWarps + (threadIdx.x >> 5)) * 512;
@@ -252,7 +259,10 @@ __global__ void __launch_bounds__(kSumWarps * 32) sample_summary_kernel(const Sa
 __global__ void __launch_bounds__(kSumWarps * 32) sample_summary_wide_kernel(const SampleParams P, int segments, int blocks) {
     pdl_trigger();
     pdl_wait();
-    if (blockIdx.x == 0 && threadIdx.x == 0) P.queue[0] = 0;
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+        P.queue[0] = 0;
+        if (P.nucleus) P.nucleus[0] = 0;
+    }
     const int lane = threadIdx.x & 31;
     const int r = (int)(blockIdx.x / (unsigned)segments);
     const int warp = (int)(blockIdx.x - (unsigned)r * segments) * kSumWarps + (threadIdx.x >> 5);
@@ -324,16 +334,6 @@ struct BlockScratch {
 };
 // Sum over the block of an int / double, given to every thread; `flip` alternates two buffers so
 // that one barrier per call is enough.
-__device__ __forceinline__ int block_sum_int(int v, BlockScratch& s, int& flip) {
-    v = __reduce_add_sync(0xffffffffu, v);
-    flip ^= 1;
-    if ((threadIdx.x & 31) == 0) s.u[flip][threadIdx.x >> 5] = (uint32_t)v;
-    __syncthreads();
-    int t = 0;
-#pragma unroll
-    for (int i = 0; i < kWarps; ++i) t += (int)s.u[flip][i];
-    return t;
-}
 __device__ __forceinline__ uint32_t block_max(uint32_t v, BlockScratch& s, int& flip) {
     v = __reduce_max_sync(0xffffffffu, v);
     flip ^= 1;
@@ -575,8 +575,11 @@ __global__ void __launch_bounds__(kThreads) sample_finish_kernel(const SamplePar
     }
     const float m = key_logit(top);
     const double u = row_uniform(P, r);
-    auto leave = [&](double mass) {  // to the general kernel
-        if (threadIdx.x == 0) P.rowmass[r] = mass, P.queue[1 + atomicAdd(P.queue, 1)] = r;
+    auto leave = [&](double mass) {  // to one of the kernels that follow
+        if (threadIdx.x != 0) return;
+        int* const queue = P.nucleus && st.mode == kTopP && st.mp == 0.0 ? P.nucleus : P.queue;
+        P.rowmass[r] = mass, P.rowkey[r] = top;
+        queue[1 + atomicAdd(queue, 1)] = r;
     };
     if (st.mode == kGeneral) {
         leave(0.0);
@@ -885,10 +888,447 @@ __global__ void __launch_bounds__(kThreads) sample_finish_kernel(const SamplePar
     }
 }
 
+// ---------------------------------------------------------------- nucleus --
+// A cluster of up to 8 CTAs takes a queued row with a top-p alone and reads it twice, from L2 where
+// the batch fits there.  No logit that weighs less than (1 - p) total / vocab is kept (all of those
+// together weigh less than what top-p may drop), so the logits from there to the highest are
+// counted in 8192 parts of even width.  A part's number times the weight of its middle is right to
+// a factor of half a part's width, so the parts where the prefix can end are known for certain:
+// some 0.1 % of the mass around it.  The second pass sums what lies above them exactly and lists
+// what lies in them; CTA 0 finds the end of the prefix in the list.  The sums of the segments (512
+// logits), with what is kept of the list, then give the pick's segment.  Weights of the list are
+// summed as integers, so that the order of the list, which the atomics decide, does not matter.
+// Rows whose list is too long (a top_p close to 1 over a flat row, or equal logits) go on to the
+// general kernel.
+//
+// Its share of a call with 64 rows of 262144 logits and a top_p around 0.9 (some twenty rows come
+// here): 53 us, of the general kernel in its place 118; 200 such rows: the call takes 260 us instead
+// of 528, one row 30 instead of 35.  What bounds it is the chain of steps of a row, about 66
+// thousand clocks of two passes (four segments of a warp one after the other in each) and seven
+// barriers of the cluster.  1024 threads with one segment in registers: with 512 threads and the
+// next segment's loads in flight, at two CTAs per SM (64 registers, spills), the call took 128 us,
+// at one 106; this way 101.
+constexpr int kMaxCluster = 16;
+constexpr int kMaxRanks = 8;   // of the nucleus kernel: a thread has one of the parts or more
+constexpr int kWide = 1024;    // its threads
+constexpr int kWideWarps = kWide / 32;
+constexpr int kParts = 8192;
+constexpr int kList = 8192;
+constexpr int kSegment = 512;      // at most kWide segments per CTA
+constexpr int kFixed = 44;         // bits of a listed weight: kList of them stay below 2^58
+constexpr int kCount = 256;      // listed logits ranked by counting
+
+struct NucleusShared {
+    union {
+        uint32_t own[kParts + 32];         // this CTA's numbers, and a lane's of what lies below
+        unsigned long long listed[kList];  // all lists: key << 32 | ~index
+    };
+    union {
+        uint32_t num[kParts];  // the row's numbers in this CTA's parts
+        uint2 list[kList];     // key, index
+    };
+    union {
+        float staged[kWideWarps][kSegment];  // a warp's segment
+        unsigned long long listed_weight[kList];
+        double weight[kSegment + kSegment / 16];  // of the pick's segment
+    };
+    double seg[kWide];  // per segment: weight above the listed parts
+    unsigned long long seg_listed[kWide];
+    unsigned long long few_weight[kWide];
+    uint16_t few[kCount];
+    double scratch[2 * kWideWarps];
+    double xpart[kMaxCluster];                // per rank: estimated weight of its parts
+    double xmass[kMaxCluster];                // per rank: weight above
+    unsigned long long xlisted[kMaxCluster];  // per rank: kept of the list
+    int xn[kMaxCluster];                      // per rank: length of the list
+    int xfirst[kMaxCluster], xlast[kMaxCluster];
+    double start;
+    unsigned long long past;
+    int n, first, last, at, nfew, fine;
+    uint32_t end_key;  // the prefix ends with this key,
+    int end_index;     // of equal ones at this index; -1: not found
+};
+
+// Out of line: for code that runs once or twice per row.
+__device__ __noinline__ double exp2_call(double d, double c) { return exp2_64(d, c); }
+template <class T>
+struct Scan {
+    T before, all;
+};
+// Sum over the threads before this one, and over all.
+template <class T>
+__device__ __noinline__ Scan<T> block_scan(T v, void* scratch) {
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    T* const sums = static_cast<T*>(scratch);
+    T x = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const T y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+    }
+    __syncthreads();
+    if (lane == 31) sums[w] = x;
+    __syncthreads();
+    T y = sums[lane];  // a warp each
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const T z = __shfl_up_sync(0xffffffffu, y, o);
+        if (lane >= o) y += z;
+    }
+    static_assert(kWideWarps == 32, "a lane per warp");
+    const T warps = __shfl_sync(0xffffffffu, y, w > 0 ? w - 1 : 0), left = __shfl_up_sync(0xffffffffu, x, 1);
+    return {(w > 0 ? warps : T(0)) + (lane > 0 ? left : T(0)), __shfl_sync(0xffffffffu, y, 31)};
+}
+
+__global__ void __launch_bounds__(kWide, 1) sample_nucleus_kernel(const SampleParams P, int vec) {
+    extern __shared__ __align__(16) uint8_t smem_raw[];
+    NucleusShared& S = *reinterpret_cast<NucleusShared*>(smem_raw);
+    cg::cluster_group cluster = cg::this_cluster();
+    const int rank = (int)cluster.block_rank(), ranks = (int)cluster.num_blocks();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    pdl_trigger();
+    pdl_wait();
+    cluster.sync();  // every CTA of the cluster runs before any reaches into another's shared memory
+    const int segments = ((P.vocab + kSegment - 1) / kSegment + ranks - 1) / ranks;  // of a CTA
+    const int first = rank * segments * kSegment;
+    const int queued = P.nucleus[0];
+#pragma unroll 1
+    for (int q = blockIdx.x / ranks; q < queued; q += gridDim.x / ranks, cluster.sync()) {
+        const int r = P.nucleus[1 + q];
+        const float* row = P.logits + (size_t)r * P.ld;
+        const float temperature = P.how.temperature ? P.how.temperature[r] : 1.f;
+        const double p = (double)P.how.top_p[r], total = P.rowmass[r], t = p * total;
+        const double c = 1.4426950408889634 / (double)temperature;
+        const double u = row_uniform(P, r);
+        const float m = key_logit(P.rowkey[r]);
+        auto leave = [&]() {
+            if (rank == 0 && threadIdx.x == 0) P.queue[1 + atomicAdd(P.queue, 1)] = r;
+        };
+        // The lowest logit of interest, rounded down (by far more than the roundings of this line).
+        const float bound = log2f((float)((1.0 - p) * total) / (float)P.vocab) - 0.01f;
+        float a = fmaf(bound * 0.6931472f, temperature, m);
+        a -= fabsf(a) * 1e-6f + fabsf(m) * 1e-6f;
+        const float scale = (float)kParts / (m - a);
+        const double part = 1.0 / (double)scale, width = c * part;  // of a part: in logits, in powers of two
+        if (!(a > -3.0e38f && m < 3.0e38f && scale > 0.f && scale < 3.0e38f && width < 1.0 / 64.0)) {
+            leave();
+            continue;
+        }
+        auto part_of = [&](float v) { return min(kParts - 1, (int)((v - a) * scale)); };
+        // Highest key of quarter `lane` of a segment (lanes 0 .. 3), from the groups.
+        auto quarter_key = [&](int s) {
+            uint32_t k = 0;
+            const int at = first + s * kSegment + lane * 128;
+            if (lane < 4 && s < segments && at < P.vocab) {
+                const int g = at >> P.gshift, end = min(P.groups, g + max(1, 128 >> P.gshift));
+#pragma unroll 1
+                for (int i = g; i < end; ++i) k = max(k, P.gkey[(size_t)r * P.groups + i]);
+            }
+            return k;
+        };
+        // f(s, quarters read, lane's 16 logits) for each of the warp's segments with a logit from `least` on.  Quarters
+        // without (by their highest key) are not read.
+        auto each_segment = [&](float least, auto f) {
+            uint32_t key = quarter_key(warp);
+#pragma unroll 1
+            for (int s = warp; s < segments; s += kWideWarps) {
+                const unsigned wanted = __ballot_sync(0xffffffffu, key_logit(key) >= least);  // (key 0 is a NaN's)
+                key = quarter_key(s + kWideWarps);
+                if (!wanted) continue;
+                float v[16];
+                const int base = first + s * kSegment;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    v[4 * i] = v[4 * i + 1] = v[4 * i + 2] = v[4 * i + 3] = -INFINITY;
+                    if (!(wanted >> i & 1u)) continue;
+                    if (vec) {
+                        const int at = base + i * 128 + lane * 4;
+                        if (at < P.vocab) {
+                            const float4 q4 = __ldg(reinterpret_cast<const float4*>(row + at));
+                            v[4 * i] = q4.x, v[4 * i + 1] = q4.y, v[4 * i + 2] = q4.z, v[4 * i + 3] = q4.w;
+                        }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (base + i * 128 + e * 32 + lane < P.vocab) v[4 * i + e] = __ldg(row + base + i * 128 + e * 32 + lane);
+                    }
+                }
+                if (P.cap > 0.f) {
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) v[k] = softcap(v[k], P.cap);
+                }
+                f(s, wanted, v);
+            }
+        };
+        {
+            uint4* const z = reinterpret_cast<uint4*>(S.own);
+#pragma unroll 1
+            for (int i = threadIdx.x; i < kParts / 4; i += kWide) z[i] = make_uint4(0, 0, 0, 0);
+        }
+        S.seg[threadIdx.x] = 0.0;
+        S.seg_listed[threadIdx.x] = 0;
+        if (threadIdx.x == 0) S.n = S.first = S.last = S.nfew = 0, S.at = S.end_index = S.fine = -1, S.past = 0;
+        __syncthreads();
+        each_segment(a, [&](int, unsigned wanted, const float (&v)[16]) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (!(wanted >> i & 1u)) continue;
+#pragma unroll
+                for (int k = 4 * i; k < 4 * i + 4; ++k)
+                    atomicAdd(&S.own[v[k] >= a ? part_of(v[k]) : kParts + lane], 1u);  // free of branches
+            }
+        });
+        cluster.barrier_arrive();
+        // This CTA's share of the parts, from the top, E per thread.
+        const int E = kParts / kWide / ranks, top = kParts - 1 - (rank * kWide + (int)threadIdx.x) * E;
+        const double step = exp2_64(-width, 1.0);
+        const double wtop = exp2_64((double)a + ((double)top + 0.5) * part - (double)m, c);
+        const double off = exp2_64(-0.51 * width, 1.0);  // a part's true weight: the estimate times off .. 1 / off
+        double x = 0.0, w = wtop;
+        cluster.barrier_wait();
+#pragma unroll 2
+        for (int e = 0; e < E; ++e, w *= step) {
+            uint32_t n = 0;
+#pragma unroll 4
+            for (int k = 0; k < ranks; ++k) n += *cluster.map_shared_rank(&S.own[top - e], k);
+            S.num[threadIdx.x * E + e] = n;
+            x += (double)n * w;
+        }
+        const Scan<double> parts = block_scan(x, S.scratch);
+        if ((int)threadIdx.x < ranks) *cluster.map_shared_rank(&S.xpart[rank], threadIdx.x) = parts.all;
+        cluster.sync();
+        double run = parts.before;
+#pragma unroll 1
+        for (int k = 0; k < rank; ++k) run += S.xpart[k];
+        int hi = -1, lo = -1;
+        w = wtop;
+#pragma unroll 1
+        for (int e = 0; e < E; ++e, w *= step) {
+            run += (double)S.num[threadIdx.x * E + e] * w;
+            if (hi < 0 && run >= t * off) hi = top - e;
+            if (lo < 0 && run * off >= t) lo = top - e;
+        }
+        hi = __reduce_max_sync(0xffffffffu, hi), lo = __reduce_max_sync(0xffffffffu, lo);
+        if (lane == 0 && hi >= 0) atomicMax(&S.last, hi);
+        if (lane == 0 && lo >= 0) atomicMax(&S.first, lo);
+        __syncthreads();
+        if ((int)threadIdx.x < ranks) {
+            *cluster.map_shared_rank(&S.xfirst[rank], threadIdx.x) = S.first;
+            *cluster.map_shared_rank(&S.xlast[rank], threadIdx.x) = S.last;
+        }
+        cluster.sync();
+        int b0 = 0, b1 = 0;  // the prefix ends in these parts
+#pragma unroll 1
+        for (int k = 0; k < ranks; ++k) b0 = max(b0, S.xfirst[k]), b1 = max(b1, S.xlast[k]);
+        // The values of the list, a float more on each side: only what is listed has to be in there.
+        const uint32_t klo = logit_key((float)((double)a + (double)b0 * part)), khi = logit_key((float)((double)a + (double)(b1 + 1) * part));
+        const float least = b0 > 0 ? key_logit(klo - 1) : a, past_list = b1 < kParts - 1 ? key_logit(khi + 1) : INFINITY;
+        each_segment(least, [&](int s, unsigned wanted, const float (&v)[16]) {
+            // What lies above is written side by side, so that full warps weigh it.
+            int count = 0;
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (!(wanted >> i & 1u)) continue;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float x = v[4 * i + e];
+                    if (!__any_sync(0xffffffffu, x >= least)) continue;
+                    const unsigned above = __ballot_sync(0xffffffffu, x >= past_list);
+                    if (x >= past_list) {
+                        S.staged[warp][count + __popc(above & ((1u << lane) - 1u))] = x;
+                    } else if (x >= least) {
+                        const int at = atomicAdd(&S.n, 1);
+                        if (at < kList)
+                            S.list[at] = make_uint2(logit_key(x), (uint32_t)(first + s * kSegment + i * 128 + (vec ? lane * 4 + e : e * 32 + lane)));
+                    }
+                    count += __popc(above);
+                }
+            }
+            if (count == 0) return;
+            __syncwarp();
+            double sum = 0.0;
+#pragma unroll 2
+            for (int j = lane; j < count; j += 32) sum += weight(S.staged[warp][j], m, c);
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            if (lane == 0) S.seg[s] = sum;
+        });
+        __syncthreads();
+        const Scan<double> segs = block_scan(S.seg[threadIdx.x], S.scratch);
+        if ((int)threadIdx.x < ranks) {
+            *cluster.map_shared_rank(&S.xmass[rank], threadIdx.x) = segs.all;
+            *cluster.map_shared_rank(&S.xn[rank], threadIdx.x) = S.n;
+        }
+        cluster.sync();
+        double above = 0.0;
+        int n = 0;
+#pragma unroll 1
+        for (int k = 0; k < ranks; ++k) above += S.xmass[k], n += S.xn[k];
+        if (n > kList) {
+            leave();
+            continue;
+        }
+        // Listed weights in units of 2^-kFixed of a power of two that none exceeds.
+        const double high = fmin((double)a + ((double)b1 + 1.01) * part, (double)m);
+        const int e2 = kFixed - (int)ceil((high - (double)m) * c);
+        const double unit = __hiloint2double((1023 - e2) << 20, 0), per = __hiloint2double((1023 + e2) << 20, 0);
+        auto fixed = [&](uint32_t key) {
+            const float v = key_logit(key);
+            return (unsigned long long)((v == m ? 1.0 : exp2_call((double)v - (double)m, c)) * per);
+        };
+        if (rank == 0) {
+#pragma unroll 1
+            for (int j = threadIdx.x; j < n; j += kWide) {
+                int i = j, k = 0;
+                while (i >= S.xn[k]) i -= S.xn[k++];
+                const uint2 f = *cluster.map_shared_rank(&S.list[i], k);
+                S.listed[j] = (unsigned long long)f.x << 32 | (0xffffffffu - f.y);
+                S.listed_weight[j] = fixed(f.x);
+                if (j < kCount) S.few[j] = (uint16_t)j;
+            }
+            __syncthreads();
+            const double need = (t - above) * per;
+            unsigned long long past = 0;  // what the listed above those to rank weigh
+            int left = n;
+            if (n > kCount) {
+                // 512 parts of even width again: what is listed in the one where the prefix ends is ranked.
+                const float from = (float)((double)a + (double)b0 * part), fine = (float)kWide * scale / (float)(b1 + 1 - b0);
+                auto fine_of = [&](unsigned long long f) {
+                    return max(0, min(kWide - 1, (int)((key_logit((uint32_t)(f >> 32)) - from) * fine)));
+                };
+                S.few_weight[threadIdx.x] = 0;
+                __syncthreads();
+#pragma unroll 2
+                for (int j = threadIdx.x; j < n; j += kWide) atomicAdd(&S.few_weight[fine_of(S.listed[j])], S.listed_weight[j]);
+                __syncthreads();
+                const unsigned long long mine = S.few_weight[kWide - 1 - threadIdx.x];
+                const Scan<unsigned long long> sc = block_scan(mine, S.scratch);
+                if (!((double)sc.before >= need) && (double)(sc.before + mine) >= need) S.fine = kWide - 1 - (int)threadIdx.x, S.past = sc.before;
+                __syncthreads();
+                const int fine_at = S.fine;
+                past = S.past;
+#pragma unroll 1
+                for (int j = threadIdx.x; j < n; j += kWide) {
+                    if (fine_of(S.listed[j]) != fine_at) continue;
+                    const int at = atomicAdd(&S.nfew, 1);
+                    if (at < kCount) S.few[at] = (uint16_t)j;
+                }
+                __syncthreads();
+                left = S.nfew;
+            }
+            if (left <= kCount && (int)threadIdx.x < left) {
+                const int mine = S.few[threadIdx.x];
+                const unsigned long long me = S.listed[mine];
+                unsigned long long upto = past;
+#pragma unroll 4
+                for (int j = 0; j < left; ++j) {
+                    const int i = S.few[j];
+                    upto += S.listed[i] >= me ? S.listed_weight[i] : 0ull;
+                }
+                if ((double)upto >= need && !((double)(upto - S.listed_weight[mine]) >= need)) {  // one of them at most
+#pragma unroll 1
+                    for (int k = 0; k < ranks; ++k) {
+                        *cluster.map_shared_rank(&S.end_key, k) = (uint32_t)(me >> 32);
+                        *cluster.map_shared_rank(&S.end_index, k) = (int)(0xffffffffu - (uint32_t)me);
+                    }
+                }
+            }
+        }
+        cluster.sync();
+        const uint32_t end_key = S.end_key;
+        const int end_index = S.end_index;
+        if (end_index < 0) {
+            leave();
+            continue;
+        }
+        unsigned long long listed = 0;
+#pragma unroll 1
+        for (int j = threadIdx.x; j < S.n; j += kWide) {
+            const uint2 f = S.list[j];
+            if (f.x > end_key || (f.x == end_key && (int)f.y <= end_index)) {
+                const unsigned long long y = fixed(f.x);
+                listed += y;
+                atomicAdd(&S.seg_listed[((int)f.y - first) / kSegment], y);
+            }
+        }
+        listed = block_scan(listed, S.scratch).all;
+        if ((int)threadIdx.x < ranks) *cluster.map_shared_rank(&S.xlisted[rank], threadIdx.x) = listed;
+        cluster.sync();
+        // The last CTA, segment and lane with something at or below the target hold the pick.
+        double in_rank = 0.0, upto_rank = 0.0;
+        if (lane < ranks) in_rank = S.xmass[lane] + (double)S.xlisted[lane] * unit;
+        upto_rank = in_rank;
+#pragma unroll
+        for (int o = 1; o < kMaxCluster; o <<= 1) {
+            const double z = __shfl_up_sync(0xffffffffu, upto_rank, o);
+            if (lane >= o) upto_rank += z;
+        }
+        const double kept = __shfl_sync(0xffffffffu, upto_rank, kMaxCluster - 1), target = u * kept;
+        double before = __shfl_up_sync(0xffffffffu, upto_rank, 1);
+        if (lane == 0) before = 0.0;
+        const unsigned holds = __ballot_sync(0xffffffffu, lane < ranks && in_rank > 0.0 && before <= target);
+        const int owner = 31 - __clz(holds | 1u);
+        const double start = __shfl_sync(0xffffffffu, before, owner);
+        if (owner != rank) continue;
+        const double y = S.seg[threadIdx.x] + (double)S.seg_listed[threadIdx.x] * unit;
+        before = start + block_scan(y, S.scratch).before;
+        const int held = __reduce_max_sync(0xffffffffu, y > 0.0 && before <= target ? (int)threadIdx.x : -1);
+        if (lane == 0 && held >= 0) atomicMax(&S.at, held);
+        __syncthreads();
+        if (S.at == (int)threadIdx.x) S.start = before;
+        __syncthreads();
+        if (warp == 0 && S.at >= 0) {
+            const int base = first + S.at * kSegment;
+            const float lim = key_logit(end_key);
+            auto slot = [](int i) { return i + (i >> 4); };  // (a lane's 16 are read without bank conflicts)
+            float v[16];
+#pragma unroll
+            for (int k = 0; k < 16; ++k) v[k] = base + k * 32 + lane < P.vocab ? __ldg(row + base + k * 32 + lane) : -INFINITY;
+            if (P.cap > 0.f) {
+#pragma unroll
+                for (int k = 0; k < 16; ++k) v[k] = softcap(v[k], P.cap);
+            }
+            float* const to = S.staged[kWideWarps - 1];  // (behind the weights)
+#pragma unroll
+            for (int k = 0; k < 16; ++k) to[k * 32 + lane] = v[k];
+#pragma unroll 4
+            for (int k = 0; k < 16; ++k) {
+                const int i = base + k * 32 + lane;
+                const float l = to[k * 32 + lane];
+                const double wk = weight(l, m, c);
+                S.weight[slot(k * 32 + lane)] = l > lim || (l == lim && i <= end_index) ? wk : 0.0;
+            }
+            __syncwarp();
+            double own = 0.0;
+#pragma unroll 4
+            for (int k = 0; k < 16; ++k) own += S.weight[slot(lane * 16 + k)];
+            double upto = own;
+#pragma unroll 1
+            for (int o = 1; o < 32; o <<= 1) {
+                const double z = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += z;
+            }
+            double at = S.start + (upto - own), bw = 0.0;
+            int best = -1;
+#pragma unroll 4
+            for (int k = 0; k < 16; ++k) {
+                const double wk = S.weight[slot(lane * 16 + k)];
+                if (wk > 0.0 && at <= target) best = base + lane * 16 + k, bw = wk;
+                at += wk;
+            }
+            const int pick = __reduce_max_sync(0xffffffffu, best);
+            if (best == pick && best >= 0) {
+                P.ids[r] = best;
+                if (P.probs) P.probs[r] = (float)(bw / kept);
+            }
+        }
+    }
+}
+
 // ---------------------------------------------------------------- general --
 // A cluster of up to 16 CTAs takes queued rows, each CTA with its part of the row in shared
 // memory (warps own consecutive segments of 128 * J logits).
-constexpr int kMaxCluster = 16;
 constexpr int kPick = kThreads;  // logits ranked at the end of a search
 constexpr int kWays = 4;
 constexpr int kBins = 256;
@@ -1457,19 +1897,22 @@ extern "C" g4_status g4_sample(g4_ctx* ctx, const float* logits, long long ld, i
         return g4::set_error(G4_ERR_INVALID, "g4_sample: null argument");
     g4_status st = g4::use_device(ctx);
     if (st || rows == 0) return st;
-    SampleParams P{logits, ld, rows, vocab, cap, *how, ids_out, probs_out, nullptr, nullptr, nullptr, nullptr, 2, 0};
+    SampleParams P{logits, ld, rows, vocab, cap, *how, ids_out, probs_out, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, 2, 0};
     while (((vocab + (1 << P.gshift) - 1) >> P.gshift) > kMaxGroups) ++P.gshift;
     P.groups = (vocab + (1 << P.gshift) - 1) >> P.gshift;
     const long long segments = (vocab + kSumWarps * 512 - 1) / (kSumWarps * 512);
     if (segments * rows > 0x7fffffffLL)
         return g4::set_error(G4_ERR_UNSUPPORTED, "g4_sample: %d rows of %d logits", rows, vocab);
     const size_t ng = (size_t)rows * P.groups;
-    st = g4::ensure_workspace(ctx, (ng + rows) * sizeof(double) + ng * sizeof(uint32_t) + ((size_t)rows + 1) * sizeof(int));
+    st = g4::ensure_workspace(ctx, (ng + rows) * sizeof(double) + (ng + rows) * sizeof(uint32_t) + 2 * ((size_t)rows + 1) * sizeof(int));
     if (st) return st;
     P.gmass = static_cast<double*>(ctx->ws);
     P.rowmass = P.gmass + ng;
     P.gkey = reinterpret_cast<uint32_t*>(P.rowmass + rows);
-    P.queue = reinterpret_cast<int*>(P.gkey + ng);
+    P.rowkey = P.gkey + ng;
+    P.queue = reinterpret_cast<int*>(P.rowkey + rows);
+    // With a top_k few rows are left over, and the launch would cost more than it saves.
+    if (how->top_p && !how->top_k) P.nucleus = P.queue + rows + 1;
     const int vec = reinterpret_cast<uintptr_t>(logits) % 16 == 0 && (ld % 4 == 0 || rows == 1);
     const int vec4 = vec && vocab % 4 == 0;  // every row in whole 16-byte pieces
 
@@ -1488,6 +1931,9 @@ extern "C" g4_status g4_sample(g4_ctx* ctx, const float* logits, long long ld, i
                                            (int)sizeof(FinishShared)));
         G4_CHECK_CUDA(cudaFuncSetAttribute(sample_general_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
         G4_CHECK_CUDA(cudaFuncSetAttribute(sample_general_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+        G4_CHECK_CUDA(cudaFuncSetAttribute(sample_nucleus_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                           (int)sizeof(NucleusShared)));
+        G4_CHECK_CUDA(cudaFuncSetAttribute(sample_nucleus_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
         attr_set.fetch_or(1ull << ctx->device);
     }
     if (vec4 && P.gshift >= 7) {
@@ -1507,6 +1953,17 @@ extern "C" g4_status g4_sample(g4_ctx* ctx, const float* logits, long long ld, i
     ctx->pdl = true;
     st = g4::launch(ctx, "sample_finish_kernel", sample_finish_kernel, dim3(rows), dim3(kThreads), sizeof(FinishShared), 1, P,
                     vec4);
+    if (!st && P.nucleus) {
+        // One wave of clusters, if half of the rows come there, while a CTA has 8192 logits or more (64 rows
+        // of 262144 in clusters of 8, of which a third came: 128 us, in clusters of 4: 104).
+        int per = 1;
+        while (per < kMaxRanks && (vocab > per * kWide * kSegment ||
+                                     (2LL * per * rows <= 2 * ctx->num_sms && vocab >= 2 * per * 8192)))
+            per <<= 1;
+        st = g4::launch(ctx, "sample_nucleus_kernel", sample_nucleus_kernel,
+                        dim3(std::max(1, std::min(rows, ctx->num_sms / per)) * per), dim3(kWide), sizeof(NucleusShared),
+                        per, P, vec4);
+    }
     // Only top-k, top-p and min-p can leave a row to the general kernel.
     if (!st && (how->top_k || how->top_p || how->min_p)) {
         const int clusters = std::max(1, std::min(rows, 2 * ctx->num_sms / ranks));

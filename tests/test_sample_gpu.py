@@ -279,3 +279,49 @@ def test_refusals(rt, ops):
             bad()
     ids, _ = ops.sample(x[:0], u[:0])
     assert ids.numel() == 0
+
+
+@pytest.mark.parametrize("V", [8195, 16384, 70001, 128256, 262144, 786432])
+@pytest.mark.parametrize("p", [0.6, 0.9, 0.97, 0.999])
+def test_long_nuclei(ops, V, p):
+    """Prefixes of some hundred to most of the row's logits, at flat and steep temperatures."""
+    l, _ = rows(6, V, V + 1, scale=1.5)
+    l[1] *= 0.05  # nearly flat
+    l[2] = np.round(l[2] * 8) / 8  # few values, many ties
+    l[3, V // 3:] = np.finfo(np.float32).min
+    l[4, ::2] = np.nan
+    u = np.array([0.0, 0.2, 0.5, 0.999, 1 - 2.0**-24, 0.77], np.float32)
+    check(ops, l, u, p=p)
+    check(ops, l, u[::-1].copy(), T=np.array([0.5, 3.0, 1.0, 0.02, 1.7, 40.0]), p=p)
+
+
+def test_long_nuclei_of_rounded_logits(ops):
+    """Logits on the bf16 grid lie on the borders of what the search compares them with."""
+    l, u = rows(12, 100000, 3, scale=3.0)
+    l = torch.from_numpy(l).bfloat16().float().numpy()
+    check(ops, l, u, p=np.linspace(0.3, 0.98, 12))
+    check(ops, l, u, T=1.9, p=np.linspace(0.98, 0.3, 12))
+
+
+@pytest.mark.parametrize("rows_", [1, 40, 150, 330])
+def test_long_nuclei_of_many_rows(ops, rows_):
+    l, u = rows(rows_, 20480, rows_, scale=1.0)
+    check(ops, l, u, T=np.linspace(0.2, 2.0, rows_), p=np.linspace(0.2, 0.99, rows_))
+
+
+def test_long_nuclei_of_capped_strided_rows(rt, ctx, ops):
+    """With a cap, from rows that are not 16-byte aligned, the same bits as from capped aligned ones."""
+    l, u = rows(5, 30003, 12, scale=10.0)
+    big = torch.zeros((5, 40001), device="cuda")
+    view = big[:, 3:3 + 30003]
+    view.copy_(torch.from_numpy(l))
+    U, p = torch.from_numpy(u).cuda(), torch.tensor([0.5, 0.7, 0.9, 0.95, 0.99], device="cuda")
+    got = ops.sample(view, U, top_p=p, cap=20.0)
+    flat = torch.zeros((5, 30004), device="cuda")[:, :30003]
+    capped = torch.from_numpy(l).cuda()
+    rt.call("g4_softcap", ctx.handle, C.c_void_p(capped.data_ptr()), capped.numel(), C.c_float(20.0))
+    flat.copy_(capped)
+    for x in (flat, capped):
+        want = ops.sample(x, U, top_p=p)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    check(ops, capped.cpu().numpy(), u, p=[0.5, 0.7, 0.9, 0.95, 0.99], view=capped)
