@@ -988,6 +988,7 @@ __global__ void __launch_bounds__(kWide, 1) sample_nucleus_kernel(const SamplePa
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     pdl_trigger();
     pdl_wait();
+    if ((int)blockIdx.x / ranks >= P.nucleus[0]) return;  // nothing for this cluster
     cluster.sync();  // every CTA of the cluster runs before any reaches into another's shared memory
     const int segments = ((P.vocab + kSegment - 1) / kSegment + ranks - 1) / ranks;  // of a CTA
     const int first = rank * segments * kSegment;
@@ -1812,6 +1813,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_general_kernel(const Sampl
     const int rank = (int)cluster.block_rank(), ranks = (int)cluster.num_blocks();
     pdl_trigger();
     pdl_wait();
+    if ((int)blockIdx.x / ranks >= P.queue[0]) return;  // nothing for this cluster
     cluster.sync();  // every CTA of the cluster runs before any writes to another's shared memory
     General g{P, S, chunk, cluster, rank, ranks, J, 0, 0, 0, 0.f, 0u, 0u, 0.0};
     const int queued = P.queue[0];
