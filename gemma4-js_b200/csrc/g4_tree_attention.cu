@@ -25,6 +25,7 @@ using namespace g4dev;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kTile = 128;        // keys per tile = MMA N of the scores
 constexpr int kRowsPerCta = 128;  // MMA M
+constexpr int kRest = 3 * 1024;   // shared memory besides Q and the ring
 // Four threads per query row, each with a quarter of a tile's keys (scores are read once and stay in
 // registers) and of O's columns: four warps per scheduler hide each other's latencies.  32 sequences
 // of 512 rows over 4160 keys at hd 256: 59.6 us, with two threads per row (scores read twice) 60.6; one
@@ -64,7 +65,7 @@ struct TreeCfg {
     static constexpr int VKEYS = kTile / VGRAN;                // keys per V granule
     static constexpr int VBOX = VKEYS * 128;                   // bytes of a V box
     static constexpr int SLOTS = SLOT == 16384 ? 8 : (229376 - QBYTES) / SLOT;
-    static constexpr int SMEM = QBYTES + SLOTS * SLOT + 3072;  // the rest: TreeShared
+    static constexpr int SMEM = QBYTES + SLOTS * SLOT + kRest;  // the rest: TreeShared
     static_assert(SMEM <= 232448, "shared memory");
     static_assert(!kPair || HD >= 128, "half of V is whole 64-column chunks");
 };
@@ -91,7 +92,7 @@ struct TreeShared {
     int mx[3][kRowsPerCta];  // a row's maximum, ordered as integers (three tiles in turn)
 };
 
-static_assert(sizeof(TreeShared) <= 3072, "shared memory");
+static_assert(sizeof(TreeShared) <= kRest, "shared memory");
 
 __device__ __forceinline__ float ex2(float x) {  // 2^x to 2^-22, 0 for -inf
     float y;
