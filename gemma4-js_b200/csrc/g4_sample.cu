@@ -381,63 +381,30 @@ __device__ __forceinline__ double block_prefix(double v, BlockScratch& s, int& f
     return before + left;
 }
 
-// Bitonic sort of n2 = a power of two up to kThreads * E 64-bit values in shared memory, largest
-// first.  Values stay in registers (value e * kThreads + t in thread t): partners less than 32 away
-// come by shuffle, more than the block away from the thread itself, the others through `a` and
-// `b` in turn, one barrier a step (18 of the 66 steps of 2048 values).
-template <int E>
+// Bitonic sort of n2 = a power of two up to kThreads 64-bit values in shared memory, largest first.
+// Values stay in registers: partners less than 32 away come by shuffle, the others through `a` and
+// `b` in turn, one barrier a step.
 __device__ __forceinline__ void block_sort_desc(unsigned long long* a, unsigned long long* b, int n2) {
     const int t = threadIdx.x;
-    unsigned long long v[E];
     __syncthreads();
-#pragma unroll
-    for (int e = 0; e < E; ++e) v[e] = e * kThreads + t < n2 ? a[e * kThreads + t] : 0ull;
+    unsigned long long v = t < n2 ? a[t] : 0ull;
     bool second = true;  // the buffer that may be written: a's values have been read after the next barrier
     for (int size = 2; size <= n2; size <<= 1) {
         for (int step = size >> 1; step > 0; step >>= 1) {
-            if (step >= kThreads) {
-                const int de = step / kThreads;
-#pragma unroll
-                for (int e = 0; e < E; ++e) {
-#pragma unroll
-                    for (int f = e + 1; f < E; ++f) {
-                        if (f != (e ^ de)) continue;
-                        const bool desc = ((e * kThreads + t) & size) == 0;
-                        if ((v[e] < v[f]) == desc) {
-                            const unsigned long long x = v[e];
-                            v[e] = v[f], v[f] = x;
-                        }
-                    }
-                }
-                continue;
-            }
             unsigned long long* const buf = second ? b : a;
             if (step >= 32) {
-#pragma unroll
-                for (int e = 0; e < E; ++e) buf[e * kThreads + t] = v[e];
+                buf[t] = v;
                 __syncthreads();
                 second = !second;
             }
-#pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const int i = e * kThreads + t;
-                const unsigned long long o = step >= 32 ? buf[i ^ step] : __shfl_xor_sync(0xffffffffu, v[e], step);
-                const bool larger = ((i & size) == 0) == ((i & step) == 0);  // this one keeps the larger
-                v[e] = (o > v[e]) == larger ? o : v[e];
-            }
+            const unsigned long long o = step >= 32 ? buf[t ^ step] : __shfl_xor_sync(0xffffffffu, v, step);
+            const bool larger = ((t & size) == 0) == ((t & step) == 0);  // this one keeps the larger
+            v = (o > v) == larger ? o : v;
         }
     }
     __syncthreads();
-#pragma unroll
-    for (int e = 0; e < E; ++e)
-        if (e * kThreads + t < n2) a[e * kThreads + t] = v[e];
+    if (t < n2) a[t] = v;
     __syncthreads();
-}
-template <int E>
-__device__ __forceinline__ void block_sort_desc_any(unsigned long long* a, unsigned long long* b, int n2) {
-    if (n2 <= kThreads) block_sort_desc<1>(a, b, n2);
-    else if (n2 <= 2 * kThreads) block_sort_desc<2>(a, b, n2);
-    else block_sort_desc<E>(a, b, n2);
 }
 __device__ __forceinline__ int pow2_at_least(int n) { return n <= 2 ? 2 : 1 << (32 - __clz(n - 1)); }
 
@@ -458,7 +425,49 @@ struct FinishShared {
     int n, ng, kept, found, pick;
     uint32_t hist[256], found_above, found_in;
     int rank[kFew];
+    int begin[kThreads + 1], cursor[kThreads];
 };
+
+// Sorts S.cand[0 .. n), n <= kCand distinct values, largest first.  bin(value) in [0, kThreads) falls
+// as the value rises: values go to their bin's place, and inside it (a handful, if bin spreads them)
+// each counts the larger ones.  Two bitonic sorts of 2048 values in its place took 50 us of a row.
+template <class Bin>
+__device__ __forceinline__ void bin_sort_desc(FinishShared& S, int n, Bin bin) {
+    const int t = threadIdx.x, lane = t & 31;
+    S.cursor[t] = 0;
+    __syncthreads();
+    for (int i = t; i < n; i += kThreads) atomicAdd(&S.cursor[bin(S.cand[i])], 1);
+    __syncthreads();
+    const int own = S.cursor[t];
+    int x = own;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+    }
+    if (lane == 31) S.begin[t >> 5] = x;
+    __syncthreads();
+    int before = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) before += w < t >> 5 ? S.begin[w] : 0;
+    __syncthreads();
+    S.begin[t] = S.cursor[t] = before + x - own;
+    if (t == 0) S.begin[kThreads] = n;
+    __syncthreads();
+    for (int i = t; i < n; i += kThreads) {
+        const unsigned long long v = S.cand[i];
+        S.cand2[atomicAdd(&S.cursor[bin(v)], 1)] = v;
+    }
+    __syncthreads();
+    for (int i = t; i < n; i += kThreads) {
+        const unsigned long long v = S.cand2[i];
+        const int b = bin(v), from = S.begin[b], to = S.begin[b + 1];
+        int larger = 0;
+        for (int j = from; j < to; ++j) larger += S.cand2[j] > v;
+        S.cand[from + larger] = v;
+    }
+    __syncthreads();
+}
 
 // Lists the logits of four that are `least` or more.  Out of line: code that runs once costs its
 // fetches, not its instructions.
@@ -509,8 +518,9 @@ __device__ __forceinline__ void finish_few(const SampleParams& P, FinishShared& 
         return;
     }
     // kept: the shortest prefix of the filters.
-    if (t < limit && ((st.p < 1.0 && run >= need) || (t + 1 < limit && st.mp > 0.0 && S.w[t + 1] < st.mp)))
-        atomicMin(&S.kept, t + 1);
+    const unsigned ends = __ballot_sync(
+        0xffffffffu, t < limit && ((st.p < 1.0 && run >= need) || (t + 1 < limit && st.mp > 0.0 && S.w[t + 1] < st.mp)));
+    if (ends && (t & 31) == 0) atomicMin(&S.kept, t + __ffs(ends));
     __syncthreads();
     const int kept = S.kept;
     if (t == kept - 1) S.zk = run;
@@ -525,14 +535,16 @@ __device__ __forceinline__ void finish_few(const SampleParams& P, FinishShared& 
     }
     __syncthreads();
     const double target = u * S.zk;
-    int mine = -1;
+    int mine = -1, at = -1;
     if (t < kept && w > 0.0) {
         double s0 = 0.0;
         for (int q = 0; q < parts; ++q) s0 += before[q * n2 + t];
         mine = (int)(0xffffffffu - (uint32_t)sorted[t]);
         // the highest index with no more than the target before it
-        if (s0 <= target) atomicMax(&S.pick, mine);
+        if (s0 <= target) at = mine;
     }
+    at = __reduce_max_sync(0xffffffffu, at);
+    if (at >= 0 && (t & 31) == 0) atomicMax(&S.pick, at);
     __syncthreads();
     if (mine >= 0 && mine == S.pick) {
         P.ids[r] = mine;
@@ -600,10 +612,8 @@ __global__ void __launch_bounds__(kThreads) sample_finish_kernel(const SamplePar
         const double target = u * total;
         // The thread whose groups hold the target; its first group past it (the last positive one
         // where rounding leaves none).
-        if (own > 0.0 && before <= target) {
-            // the highest such thread wins
-            atomicMax(&S.ng, (int)threadIdx.x + 1);
-        }
+        const unsigned holds = __ballot_sync(0xffffffffu, own > 0.0 && before <= target);  // the highest such thread wins
+        if (holds && (threadIdx.x & 31) == 0) atomicMax(&S.ng, (int)threadIdx.x + 32 - __clz(holds));
         __syncthreads();
         if (S.ng == (int)threadIdx.x + 1) {
             double run = before;
@@ -659,6 +669,7 @@ __global__ void __launch_bounds__(kThreads) sample_finish_kernel(const SamplePar
     const double c = st.scale();
     uint32_t bound;
     double total = 0.0;
+    const bool whole = P.vocab <= kCand;  // every logit may be a candidate
     if (st.mode == kMinP) {
         // The lowest key that weighs mp or more (w falls with the key): every thread tries one of 512
         // keys of what is left.
@@ -699,11 +710,11 @@ __global__ void __launch_bounds__(kThreads) sample_finish_kernel(const SamplePar
             }
             total = block_sum(own, S.scratch, flip);
             const double fixed = st.p * total * 1048576.0 + kMaxGroups;
-            if (fixed > 2147483648.0) {  // more than all maxima can weigh
+            if (fixed > 2147483648.0 && !whole) {  // more than all maxima can weigh
                 leave(total);
                 return;
             }
-            need = (uint32_t)fixed;
+            need = (uint32_t)fmin(fixed, 4294967295.0);
         }
         uint32_t lo = low, hi = top + 1, above = 0;
         bool enough = false;
@@ -769,7 +780,7 @@ __global__ void __launch_bounds__(kThreads) sample_finish_kernel(const SamplePar
             above = S.found_above;
             if (shift == 0 || above + S.found_in <= need + need / 8 + (st.mode == kTopK ? 4 : 0)) done = true;
         }
-        if (!enough && st.mode == kTopP) {
+        if (!enough && st.mode == kTopP && !whole) {
             leave(total);
             return;
         }
@@ -820,9 +831,13 @@ __global__ void __launch_bounds__(kThreads) sample_finish_kernel(const SamplePar
         finish_few(P, S, st, r, n, m, c, u, total, flip, leave);
         return;
     }
-    int n2 = pow2_at_least(n);
-    for (int i = n + threadIdx.x; i < n2; i += kThreads) S.cand[i] = 0ull;
-    block_sort_desc_any<kCand / kThreads>(S.cand, S.cand2, n2);
+    uint32_t least_key = 0;
+    for (int i = threadIdx.x; i < n; i += kThreads) least_key = max(least_key, ~(uint32_t)(S.cand[i] >> 32));
+    const float lowest = key_logit(~block_max(least_key, S.scratch, flip)), parts = (float)kThreads / (m - lowest);
+    bin_sort_desc(S, n, [&](unsigned long long v) {
+        if (!(parts < 3.0e38f)) return 0;  // equal logits, or infinite ones
+        return kThreads - 1 - min(kThreads - 1, (int)((key_logit((uint32_t)(v >> 32)) - lowest) * parts));
+    });
     // Ranks 4t .. 4t + 3: weights, their running sum and where it ends the prefix.
     constexpr int E = kCand / kThreads;
     const int limit = st.mode == kTopK ? min(st.k, n) : n;
@@ -831,7 +846,7 @@ __global__ void __launch_bounds__(kThreads) sample_finish_kernel(const SamplePar
     for (int e = 0; e < E; ++e) {
         const int i = threadIdx.x * E + e;
         w[e] = i < limit ? weight(key_logit((uint32_t)(S.cand[i] >> 32)), m, c) : 0.0;
-        if (i < n2) S.w[i] = w[e];
+        if (i < n) S.w[i] = w[e];
         own += w[e];
     }
     double run = block_prefix(own, S.scratch, flip, &all);
@@ -844,22 +859,25 @@ __global__ void __launch_bounds__(kThreads) sample_finish_kernel(const SamplePar
     // kept: the longest prefix that the filters leave.
     if (threadIdx.x == 0) S.kept = limit;
     __syncthreads();
+    int upto = limit;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
         const int i = threadIdx.x * E + e;
         run += w[e];
         if (i < limit && ((st.p < 1.0 && run >= need) || (i + 1 < limit && st.mp > 0.0 && S.w[i + 1] < st.mp)))
-            atomicMin(&S.kept, i + 1);
+            upto = min(upto, i + 1);
     }
+    upto = __reduce_min_sync(0xffffffffu, upto);
+    if ((threadIdx.x & 31) == 0 && upto < limit) atomicMin(&S.kept, upto);
     __syncthreads();
     const int kept = S.kept;
     // The kept ones in index order.
-    n2 = pow2_at_least(kept);
-    for (int i = threadIdx.x; i < n2; i += kThreads) {
-        // ~index << 32 | position: largest first is lowest index first
-        S.cand[i] = i < kept ? (S.cand[i] & 0xffffffffull) << 32 | (unsigned)i : 0ull;
-    }
-    block_sort_desc_any<kCand / kThreads>(S.cand, S.cand2, n2);
+    for (int i = threadIdx.x; i < kept; i += kThreads)
+        S.cand[i] = (S.cand[i] & 0xffffffffull) << 32 | (unsigned)i;  // ~index << 32 | position: lowest index first
+    __syncthreads();
+    bin_sort_desc(S, kept, [&](unsigned long long v) {
+        return (int)((unsigned long long)(0xffffffffu - (uint32_t)(v >> 32)) * kThreads / (unsigned)P.vocab);
+    });
     own = 0.0;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
@@ -879,7 +897,8 @@ __global__ void __launch_bounds__(kThreads) sample_finish_kernel(const SamplePar
         if (w[e] > 0.0 && run <= target) mine = threadIdx.x * E + e;
         run += w[e];
     }
-    if (mine >= 0) atomicMax(&S.n, mine);
+    const int last = __reduce_max_sync(0xffffffffu, mine);
+    if ((threadIdx.x & 31) == 0 && last >= 0) atomicMax(&S.n, last);
     __syncthreads();
     if (mine >= 0 && mine == S.n) {
         const unsigned long long c = S.cand[mine];
@@ -1659,7 +1678,7 @@ struct General {
             } else {
                 const int n2 = pow2_at_least(n);
                 for (int i = n + t0; i < n2; i += kThreads) S.cand[i] = 0ull;
-                block_sort_desc<1>(S.cand, S.cand2, n2);
+                block_sort_desc(S.cand, S.cand2, n2);
             }
             const double w = t0 >= n ? 0.0 : count ? 1.0 : weight(key_logit((uint32_t)(S.cand[t0] >> 32)), m, c);
             if (t0 == 0) S.at = n;
