@@ -325,3 +325,22 @@ def test_long_nuclei_of_capped_strided_rows(rt, ctx, ops):
         want = ops.sample(x, U, top_p=p)
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
     check(ops, capped.cpu().numpy(), u, p=[0.5, 0.7, 0.9, 0.95, 0.99], view=capped)
+
+
+@pytest.mark.parametrize("V", [257, 300, 512, 513, 2047, 2048, 2049])
+def test_rankings_of_some_hundred_candidates(ops, V):
+    """Rows that are ranked whole: even, crowded at one end, of few values, equal, masked, infinite."""
+    rng = np.random.default_rng(V)
+    l = rng.standard_normal((9, V)).astype(np.float32)
+    l[1] = -np.exp(4 * rng.random(V))
+    l[2] = np.round(l[2] * 4) / 4
+    l[3] = 1.5
+    l[4, : V - 3] = np.finfo(np.float32).min
+    l[5, ::2] = -np.inf
+    l[6, 5] = l[6, V - 1] = np.inf
+    l[7] = np.sort(l[7])[::-1] * 1e-30
+    l[8, rng.integers(0, V, 20)] = np.nan
+    u = np.array([0.1, 0.5, 0.9, 0.3, 0.7, 0.999, 0.6, 0.0, 0.45], np.float32)
+    for kw in ({"p": 0.97}, {"p": 0.9999, "T": 50.0}, {"k": V - 1}, {"k": 290, "p": 0.99}, {"mp": 1e-4}, {"mp": 0.9, "T": 20.0},
+               {"k": V // 2 + 1, "p": 0.8, "mp": 1e-3, "T": 3.0}):
+        check(ops, l, u, **kw)
