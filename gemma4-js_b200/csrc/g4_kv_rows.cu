@@ -11,17 +11,18 @@ namespace {
 
 using namespace g4dev;
 
-constexpr int kMaxCaches = 48;  // caches per launch (40 B each, of the 4 KiB of arguments)
+constexpr int kMaxCaches = 48;  // caches per launch (32 B each, of the 4 KiB of arguments)
 constexpr int kMaxPairs = 128;  // fork pairs per launch
 
 struct CacheRef {
     uint16_t *k, *v;
     int hd, stride;    // stride: rows per sequence
     int ring, mirror;  // ring caches: position p in slot p % ring, slots below mirror again at ring + slot
-    int limit;         // positions run below this
 };
 struct CacheTable {
     CacheRef c[kMaxCaches];
+    int limit;     // positions run below this in every cache of the call (also those of other launches):
+    int smallest;  // and its smallest ring: a sequence is moved in all caches or in none
 };
 __device__ __forceinline__ uint4* row_ptr(const CacheRef& c, int is_v, int seq, int slot) {
     return reinterpret_cast<uint4*>((is_v ? c.v : c.k) + ((size_t)seq * c.stride + slot) * c.hd);
@@ -94,7 +95,7 @@ __global__ void __launch_bounds__(128) kv_compact_kernel(const __grid_constant__
     if (len > 0) {
         const int last = __shfl_sync(0xffffffffu, len <= 32 ? p0 : p1, (len - 1) & 31);
         const long long end = (long long)base + last;
-        ok = ok && end < c.limit && (!c.ring || nodes <= c.ring);
+        ok = ok && end < table.limit && nodes <= table.smallest;
     }
     if (!__all_sync(0xffffffffu, ok)) {
         if (lane == 0) raise_error(err, G4_DEVERR_BAD_INDEX);
@@ -152,7 +153,7 @@ __global__ void __launch_bounds__(kForkThreads) kv_fork_kernel(const __grid_cons
     const CacheRef c = table.c[which >> 1];
     const int src = pairs.src[grp], d0 = pairs.first[grp], d1 = pairs.first[grp + 1];
     const int len = seq_pos[src];
-    if (len < 0 || len > c.limit) {
+    if (len < 0 || len > table.limit) {
         if (threadIdx.x == 0) raise_error(err, G4_DEVERR_BAD_INDEX);
         return;
     }
@@ -208,11 +209,17 @@ g4_status check_caches(const char* name, const g4_ctx* ctx, g4_kv* const* kvs, i
 
 // Up to kMaxCaches caches from kvs[first].
 int fill_table(CacheTable* t, g4_kv* const* kvs, int first, int nkv, int seq_stride) {
+    t->limit = t->smallest = 0x7fffffff;
+    for (int i = 0; i < nkv; ++i) {
+        const int limit = kvs[i]->ring ? kvs[i]->capacity : seq_stride;
+        t->limit = limit < t->limit ? limit : t->limit;
+        if (kvs[i]->ring && kvs[i]->ring < t->smallest) t->smallest = kvs[i]->ring;
+    }
     int n = 0;
     for (; n < kMaxCaches && first + n < nkv; ++n) {
         const g4_kv* kv = kvs[first + n];
-        t->c[n] = kv->ring ? CacheRef{kv->k, kv->v, kv->hd, kv->seq_rows, kv->ring, kv->mirror, kv->capacity}
-                           : CacheRef{kv->k, kv->v, kv->hd, seq_stride, 0, 0, seq_stride};
+        t->c[n] = kv->ring ? CacheRef{kv->k, kv->v, kv->hd, kv->seq_rows, kv->ring, kv->mirror}
+                           : CacheRef{kv->k, kv->v, kv->hd, seq_stride, 0, 0};
     }
     return n;
 }

@@ -435,8 +435,8 @@ g4_status g4_tree_accept(g4_ctx* ctx, const g4_tree* tree, int nseq, const int32
  * cache once; linear caches with seq_stride rows per sequence, ring caches with their own):
  * for j < accepted[s], position seq_pos[seq] + j <- position seq_pos[seq] + path[s * nodes + j],
  * seq = seq_base + s.  path must rise strictly below `nodes` (g4_tree_accept's does): a sequence
- * whose path does not, or whose drafted rows lie outside its cache, is left as it is and raises
- * G4_DEVERR_BAD_INDEX.  Advance seq_pos afterwards (g4_advance_positions_each).  The length that
+ * whose path does not, or whose drafted rows lie outside one of the caches, is left as it is in
+ * all of them and raises G4_DEVERR_BAD_INDEX.  Advance seq_pos afterwards (g4_advance_positions_each).  The length that
  * g4_kv_append keeps is not touched. */
 g4_status g4_kv_compact(g4_ctx* ctx, g4_kv* const* kvs, int nkv, int seq_stride, const int32_t* seq_pos, int seq_base,
                         int nseq, int nodes, const int32_t* path, const int32_t* accepted);
@@ -444,7 +444,7 @@ g4_status g4_kv_compact(g4_ctx* ctx, g4_kv* const* kvs, int nkv, int seq_stride,
  * cache of a host array `kvs`: the seq_pos[src] positions that the source holds (a ring cache's
  * last ones), and seq_pos[dst] = seq_pos[src].  What the destinations held behind them stays.
  * A destination may appear once and not among the sources (G4_ERR_INVALID).  A source position
- * outside its cache raises G4_DEVERR_BAD_INDEX and copies nothing. */
+ * outside one of the caches raises G4_DEVERR_BAD_INDEX and copies nothing of that source. */
 g4_status g4_kv_fork(g4_ctx* ctx, g4_kv* const* kvs, int nkv, int seq_stride, int32_t* seq_pos, const int32_t* src,
                      const int32_t* dst, int n);
 /* seq_pos[seq_base + s] += by[s] for s < nseq (by on the device: the accepted counts). */

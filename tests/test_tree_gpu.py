@@ -446,6 +446,31 @@ def test_fork_of_many_sequences_and_bad_positions(rt, ctx):
     assert int(pos[5]) == 20
 
 
+@pytest.mark.parametrize("what", ["compact", "fork"])
+@pytest.mark.parametrize("first", ["linear", "ring"])
+def test_rows_move_in_all_caches_or_in_none(rt, ctx, what, first):
+    """Caches of different extents: a position that only some of them hold changes none of them."""
+    S, stride, hd = 3, 40, 64
+    caches = [rt.KVCache(ctx, hd, S * stride), rt.KVCache(ctx, hd, 1000, ring=256, nseq=S)]
+    if first == "ring":
+        caches.reverse()
+    old = []
+    for c in caches:
+        for t in c.storage():
+            t.copy_(torch.randn(t.shape, device="cuda"))
+            old.append(t.clone())
+    pos = torch.tensor([39, 45, 7], dtype=torch.int32, device="cuda")
+    if what == "compact":
+        path = torch.tensor([[0, 2, -1]] * S, dtype=torch.int32, device="cuda")
+        rt.kv_compact(ctx, caches, pos, path, torch.tensor([2, 2, 0], dtype=torch.int32, device="cuda"), seq_stride=stride)
+    else:
+        rt.kv_fork(ctx, caches, pos, [1], [2], seq_stride=stride)
+    with pytest.raises(rt.G4Error):
+        ctx.check_device()
+    assert all(torch.equal(a, b) for a, b in zip(old, [t for c in caches for t in c.storage()]))
+    assert pos.tolist() == [39, 45, 7]
+
+
 def test_advance_each(rt, ctx):
     pos = torch.tensor([5, 6, 7, 8], dtype=torch.int32, device="cuda")
     by = torch.tensor([2, 0], dtype=torch.int32, device="cuda")
