@@ -344,3 +344,25 @@ def test_rankings_of_some_hundred_candidates(ops, V):
     for kw in ({"p": 0.97}, {"p": 0.9999, "T": 50.0}, {"k": V - 1}, {"k": 290, "p": 0.99}, {"mp": 1e-4}, {"mp": 0.9, "T": 20.0},
                {"k": V // 2 + 1, "p": 0.8, "mp": 1e-3, "T": 3.0}):
         check(ops, l, u, **kw)
+
+
+def test_two_contexts_at_once(rt, ops):
+    """Calls of two contexts on streams of their own, in flight together: the bits of one after the other."""
+    sides = [(rt.Context(0), torch.cuda.Stream()) for _ in range(2)]
+    data = []
+    for i, kw in enumerate(({"top_p": 0.9}, {"top_k": 3000, "min_p": 0.01})):
+        l, u = rows(30, 90000 + i, 50 + i, scale=1.2)
+        x, U = torch.from_numpy(l).cuda(), torch.from_numpy(u).cuda()
+        kw = {k: torch.full((30,), v, dtype=torch.int32 if k == "top_k" else torch.float32, device="cuda") for k, v in kw.items()}
+        data.append((x, U, kw, ops.sample(x, U, **kw)))
+    torch.cuda.synchronize()
+    got = [[], []]
+    for (c, s), _ in zip(sides, data):
+        c.set_stream(s)
+    for _ in range(20):
+        for i, (x, U, kw, _) in enumerate(data):
+            got[i].append(rt.GPUOps(sides[i][0]).sample(x, U, **kw))
+    torch.cuda.synchronize()
+    for i, (_, _, _, want) in enumerate(data):
+        for ids, probs in got[i]:
+            assert torch.equal(ids, want[0]) and torch.equal(probs, want[1])

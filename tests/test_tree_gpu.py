@@ -515,3 +515,30 @@ def test_refusals(rt, ctx, ops):
             f()
             pytest.fail(f"case {i} was not refused")
     assert ctx.check_device() == 0
+
+
+def test_two_contexts_at_once(rt, ctx, ops):
+    """Split and joined attention of two contexts on streams of their own, in flight together."""
+    d = lambda a: torch.tensor(a, dtype=torch.int32, device="cuda")  # noqa: E731
+    sides, calls = [], []
+    for i, (hd, n, H, base) in enumerate(((256, 8, 8, 5000), (512, 27, 7, 9000))):
+        c = rt.Context(0)
+        cache = rt.KVCache(c, hd, base + n)
+        for t in cache.storage():
+            t.copy_(torch.randn(t.shape, device="cuda"))
+        q = (torch.randn((1, n, H, hd), device="cuda") / hd**0.5).bfloat16()
+        args = (q, cache, d([base]), d(random_tree(np.random.default_rng(i), n)))
+        torch.cuda.synchronize()
+        c_ops = rt.GPUOps(c)
+        want = c_ops.attentionTree(*args)
+        torch.cuda.synchronize()
+        c.set_stream(torch.cuda.Stream())
+        sides.append(c)
+        calls.append((c_ops, args, want))
+    got = [[o.attentionTree(*a) for o, a, _ in calls] for _ in range(20)]
+    torch.cuda.synchronize()
+    for c in sides:
+        c.check_device()
+    for pair in got:
+        for out, (_, _, want) in zip(pair, calls):
+            assert torch.equal(out, want)
