@@ -1364,7 +1364,7 @@ struct GeneralShared {
     double red[kWarps][kWays];
     int redn[kWarps][kWays];
     uint32_t hist[kMaxCluster][kBins];  // per rank: number (at most 49152) and mean place of a part's logits
-    uint32_t own_hist[kBins], own_place[kBins];
+    uint32_t own_hist[kBins + 32], own_place[kBins + 32];  // the last 32: a lane's of what lies outside
     double above, past_at, n_at, n_b0, n_b1;
     float found_v;
     int found_idx, ncand, at, b0, b1, verdict;
@@ -1497,14 +1497,17 @@ struct General {
             if (threadIdx.x == 0) S.at = -1, S.b0 = kBins, S.b1 = -1;
             __syncthreads();
             each([&](int i, const float (&v)[4]) {
+                int at[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (v[e] >= a && v[e] <= b && inside(v[e], i + e, lim)) {
-                        const int at = bin(v[e]);
-                        atomicAdd(&S.own_hist[at], 1u);
-                        // its place in the part, in 1/32768
-                        if (!count) atomicAdd(&S.own_place[at], (uint32_t)(((v[e] - a) * scale - (float)at) * 32768.f));
-                    }
+                for (int e = 0; e < 4; ++e) {  // free of branches
+                    at[e] = v[e] >= a && v[e] <= b && inside(v[e], i + e, lim) ? bin(v[e]) : kBins + (int)(threadIdx.x & 31);
+                    atomicAdd(&S.own_hist[at[e]], 1u);
+                }
+                if (!count) {  // its place in the part, in 1/32768
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        atomicAdd(&S.own_place[at[e]], (uint32_t)(((v[e] - a) * scale - (float)at[e]) * 32768.f));
+                }
             });
             if (step > 0) cluster.sync();  // the last step's histograms have been read
             __syncthreads();
