@@ -758,9 +758,10 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
 }
 
 // Joins the splits of a row: out = sum_i 2^(mu_i - mu) O_i / sum_i 2^(mu_i - mu) l_i.  One CTA per
-// row and HDV columns, a thread per two columns.  The splits' (mu, l) are read at once, then every
-// split's columns independently: two round trips.  A split that saw none of the row's keys has
-// l = 0 and is left out (its O was not written).
+// row and HDV columns, a thread per two columns.  The splits' (mu, l) and the first 16 splits'
+// columns are read at once: one round trip (columns after the factors: 1.4 us more of the 15.5 us of
+// one sequence's 8 nodes over 4096 keys).  A split that saw none of the row's keys has l = 0 and is
+// left out (its O was not written).
 constexpr int kMaxSplits = 160;
 template <int HD>
 __global__ void __launch_bounds__(TreeCfg<HD, false>::HDV / 2) tree_combine_kernel(const TreeAttnParams p) {
@@ -773,6 +774,13 @@ __global__ void __launch_bounds__(TreeCfg<HD, false>::HDV / 2) tree_combine_kern
     const size_t nrows = (size_t)p.nseq * p.tree.nodes * p.heads;
     const int s = (int)(row / (p.tree.nodes * p.heads)), node = (int)(row / p.heads) - s * p.tree.nodes;
     pdl_wait();
+    // The first splits' columns are on their way before it is known which of them count.
+    constexpr int B = 16;
+    const float2* o = reinterpret_cast<const float2*>(p.part_o + row * HD + vhalf * C::HDV) + threadIdx.x;
+    auto column = [&](int i) { return i < p.nsplit ? __ldg(o + i * nrows * (HD / 2)) : make_float2(0.f, 0.f); };
+    float2 v[B];
+#pragma unroll
+    for (int b = 0; b < B; ++b) v[b] = column(b);
     for (int i = threadIdx.x; i < p.nsplit; i += T) ml[i] = p.part_ml[(i * C::NV + vhalf) * nrows + row];
     const int count = tree_count(p.tree, s, nullptr);
     const bool used = node < count && tree_seq_fits(p, tree_seq(p, s), count);
@@ -780,16 +788,20 @@ __global__ void __launch_bounds__(TreeCfg<HD, false>::HDV / 2) tree_combine_kern
     if (!used) return;
     float mu = -INFINITY;
     for (int i = 0; i < p.nsplit; ++i) mu = ml[i].y != 0.f ? fmaxf(mu, ml[i].x) : mu;
-    const float2* o = reinterpret_cast<const float2*>(p.part_o + row * HD + vhalf * C::HDV) + threadIdx.x;
     float l = 0.f, a0 = 0.f, a1 = 0.f;
-#pragma unroll 8
-    for (int i = 0; i < p.nsplit; ++i) {
-        const bool use = ml[i].y != 0.f;
-        const float f = use ? ex2(ml[i].x - mu) : 0.f;
-        const float2 v = use ? __ldg(o + i * nrows * (HD / 2)) : make_float2(0.f, 0.f);
-        l += f * ml[i].y;
-        a0 += f * v.x;
-        a1 += f * v.y;
+    for (int i0 = 0; i0 < p.nsplit; i0 += B) {
+        if (i0 > 0) {
+#pragma unroll
+            for (int b = 0; b < B; ++b) v[b] = column(i0 + b);
+        }
+#pragma unroll
+        for (int b = 0; b < B; ++b) {
+            if (i0 + b >= p.nsplit || ml[i0 + b].y == 0.f) continue;  // (its columns were not written)
+            const float f = ex2(ml[i0 + b].x - mu);
+            l += f * ml[i0 + b].y;
+            a0 += f * v[b].x;
+            a1 += f * v[b].y;
+        }
     }
     uint32_t w;
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(a1 / l), "f"(a0 / l));
