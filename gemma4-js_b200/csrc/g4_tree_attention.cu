@@ -816,11 +816,16 @@ g4_status launch_tree_attention_t(g4_ctx* ctx, const g4_kv* kv, TreeAttnParams p
     const int ntiles = (longest + kTile - 1) / kTile;
     const int across = (kPair ? (mtiles + 1) / 2 * 2 : mtiles) * C::NV;  // CTAs of a sequence and split
     const long long ctas = (long long)across * p.nseq;
-    // Split the keys while that adds CTAs to SMs without one, at three tiles or more per split: a
-    // split costs its CTA's start and drain (about three tiles' time) and the join.  One sequence
-    // of 8 nodes over 4096 keys: 15.0 us at two tiles, 15.3 at three, 19.1 at six; 64 sequences
-    // with a window of 512 (five tiles): 28.6 us in two splits, 19.9 whole.
-    const int nsplit = (int)std::max<long long>(1, std::min<long long>({ctx->num_sms / ctas, ntiles / 3, kMaxSplits}));
+    // Split the keys while that adds CTAs to SMs without one: down to one tile per split up to 16
+    // splits (which the join reads in one round trip), then to two.  One sequence of 8 nodes over 4096
+    // keys: 14.1 us at one tile, 13.6 at two, 14.3 at three; 8 sequences with a window of 512 (five
+    // tiles): 12.9, 16.7 and 18.0.  A split costs a start, a drain, the join and the partial rows'
+    // way to L2 and back, so it has to save four tiles: 64 sequences of 16 nodes with a window of 512
+    // take 33.5 us in two splits (two tiles saved), 19.7 whole, 32 of them 23.6 in four (three saved)
+    // and 19.0, 16 of them 16.9 in five (four saved) and 18.9.
+    int nsplit = (int)std::max<long long>(
+        1, std::min<long long>({ctx->num_sms / ctas, std::max(ntiles / 2, std::min(ntiles, 16)), kMaxSplits}));
+    if (ntiles - (ntiles + nsplit - 1) / nsplit < 4) nsplit = 1;
     p.nsplit = nsplit;
     const size_t nrows = (size_t)p.nseq * p.tree.nodes * p.heads;
     if (nsplit > 1) {
