@@ -89,7 +89,8 @@ __device__ __forceinline__ RowSettings row_settings(const SampleParams& P, int r
     } else if (s.p <= 0.0) {
         s.k = 1, s.p = 2.0;
     }
-    s.mode = s.k > kMaxTopK ? kGeneral : s.k ? kTopK : s.p < 1.0 ? kTopP : s.mp > 0.0 ? kMinP : kAll;
+    // (a long top-k with a min-p and no top-p is the min-p's prefix, cut at k ranks)
+    s.mode = s.k > kMaxTopK ? (s.p >= 1.0 && s.mp > 0.0 ? kMinP : kGeneral) : s.k ? kTopK : s.p < 1.0 ? kTopP : s.mp > 0.0 ? kMinP : kAll;
     return s;
 }
 
@@ -490,7 +491,7 @@ __device__ __forceinline__ void finish_few(const SampleParams& P, FinishShared& 
     unsigned long long* sorted = S.cand + kFew;
     if (t < n) sorted[S.rank[t]] = S.cand[t];
     __syncthreads();
-    const int limit = st.mode == kTopK ? min(st.k, n) : n;
+    const int limit = st.k ? min(st.k, n) : n;
     const double w = t < limit ? weight(key_logit((uint32_t)(sorted[t] >> 32)), m, c) : 0.0;
     if (t < n) S.w[t] = w;
     if (t == 0) S.kept = limit;
@@ -498,7 +499,7 @@ __device__ __forceinline__ void finish_few(const SampleParams& P, FinishShared& 
     const double run = block_prefix(w, S.scratch, flip, &all) + w;
     if (st.mode != kTopP) total = all;
     const double need = st.p * total;
-    if (st.mode == kTopP && all < need) {
+    if (st.mode == kTopP && st.mp == 0.0 && all < need) {
         leave(total);
         return;
     }
@@ -655,7 +656,20 @@ __global__ void __launch_bounds__(kThreads, 2) sample_finish_kernel(const Sample
     uint32_t bound;
     double total = 0.0;
     const bool whole = P.vocab <= kCand;  // every logit may be a candidate
-    if (st.mode == kMinP) {
+    // A top-p with a min-p: either the prefix ends among the logits that weigh mp or more, or all of
+    // those are kept; no others are looked at.
+    const bool floored = st.mode == kTopP && st.mp > 0.0;
+    if (floored) {
+        const double* gm = P.gmass + (size_t)r * G;
+        double own = 0.0;
+#pragma unroll
+        for (int i = 0; i < KG; ++i) {
+            const int g = i * kThreads + threadIdx.x;
+            own += g < G ? weight(key_logit(key[i]), m, c) * gm[g] : 0.0;
+        }
+        total = block_sum(own, S.scratch, flip);
+    }
+    if (st.mode == kMinP || floored) {
         // The lowest key that weighs mp or more (w falls with the key): every thread tries one of 512
         // keys of what is left.
         uint32_t lo = kLowestKey, hi = top;  // hi keeps
@@ -843,7 +857,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_finish_kernel(const Sample
     });
     // Ranks 4t .. 4t + 3: weights, their running sum and where it ends the prefix.
     constexpr int E = kCand / kThreads;
-    const int limit = st.mode == kTopK ? min(st.k, n) : n;
+    const int limit = st.k ? min(st.k, n) : n;
     double w[E], own = 0.0, all;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
@@ -855,7 +869,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_finish_kernel(const Sample
     double run = block_prefix(own, S.scratch, flip, &all);
     if (st.mode != kTopP) total = all;
     const double need = st.p * total;
-    if (st.mode == kTopP && all < need) {
+    if (st.mode == kTopP && st.mp == 0.0 && all < need) {
         leave(total);
         return;
     }

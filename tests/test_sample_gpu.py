@@ -366,3 +366,18 @@ def test_two_contexts_at_once(rt, ops):
     for i, (_, _, _, want) in enumerate(data):
         for ids, probs in got[i]:
             assert torch.equal(ids, want[0]) and torch.equal(probs, want[1])
+
+
+@pytest.mark.parametrize("V", [300, 5001, 51815, 128256])
+def test_min_p_beside_a_long_prefix(ops, V):
+    """A min-p that ends before, inside or behind the prefix of a top-p, or of a top-k above 1024."""
+    l, u = rows(12, V, V + 7, scale=1.7)
+    l[3] = np.round(l[3] * 4) / 4
+    l[4, ::2] = np.nan
+    l[5] = 0.25
+    mp = np.array([0.5, 0.2, 0.1, 0.05, 0.02, 0.02, 0.01, 5e-3, 2e-3, 1e-3, 1e-4, 1e-6], np.float32)
+    T = np.linspace(0.4, 2.0, 12)
+    for kw in ({"p": 0.9}, {"p": np.linspace(0.1, 0.99, 12)}, {"k": 1500}, {"k": V - 1}, {"k": 3000, "p": 0.8},
+               {"k": np.linspace(1025, 9000, 12).astype(int)}):
+        check(ops, l, u, T=T, mp=mp, **kw)
+        check(ops, l, u[::-1].copy(), mp=mp[::-1].copy(), **kw)
