@@ -14,7 +14,7 @@
 //            k-th highest logit from below, so only the about k groups above it are read again
 //            (64 of 2048 groups: 32 KB of a 1 MB row) and ranked.  Rows it cannot settle that
 //            way (a nucleus of more than some thousand tokens, top-k above 1024, masses of ties)
-//            go to a queue.
+//            go to a queue, rows of one rank never.
 //   nucleus  a cluster of CTAs reads a queued row with a top-p alone twice: once to find what the
 //            prefix can end on, once for its sum and end.
 //   general  a cluster of CTAs holds a queued row in shared memory and narrows the threshold of
@@ -581,6 +581,29 @@ __global__ void __launch_bounds__(kThreads, 2) sample_finish_kernel(const Sample
     };
     if (st.mode == kGeneral) {
         leave(0.0);
+        return;
+    }
+    if (st.k == 1) {
+        // One rank: the lowest index of the highest logit, from the first group that has it.  However many
+        // share it, so no such row is left to the kernels that follow: a call with temperatures alone has none.
+        uint32_t first = 0;  // ~ the group
+#pragma unroll
+        for (int i = 0; i < KG; ++i)
+            if (key[i] == top) first = max(first, ~(uint32_t)(i * kThreads + threadIdx.x));
+        const int g = (int)~block_max(first, S.scratch, flip);
+        if (threadIdx.x < 32) {
+            for (int o = 0; o < gs; o += 32) {
+                const int i = (g << P.gshift) + o + (int)threadIdx.x;
+                const bool has = o + (int)threadIdx.x < gs && i < P.vocab && logit_key(capped(row[i], P.cap)) == top;
+                const unsigned who = __ballot_sync(0xffffffffu, has);
+                if (!who) continue;
+                if ((int)threadIdx.x == __ffs(who) - 1) {
+                    P.ids[r] = i;
+                    if (P.probs) P.probs[r] = 1.f;
+                }
+                break;
+            }
+        }
         return;
     }
     if (st.mode == kAll) {
