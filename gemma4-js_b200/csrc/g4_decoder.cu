@@ -1039,6 +1039,7 @@ __global__ void __launch_bounds__(kThreads, 1) decode_step_kernel(DParams P) {
 
 struct g4_decoder {
     g4_ctx* ctx = nullptr;
+    int device = 0;  // of ctx, which may be destroyed first
     DParams p{};
     std::vector<WPhase> ph;
     std::vector<DLayer> layers;
@@ -1132,6 +1133,7 @@ g4_status g4_decoder_create(g4_ctx* ctx, const g4_decoder_desc* desc, const g4_d
 
     g4_decoder* d = new g4_decoder();
     d->ctx = ctx;
+    d->device = ctx->device;
     const int grid = ctx->num_sms;
     d->grid = grid;
     int max_bytes = 0, kmax = H, hdmax = 0, cap = 1 << 30;
@@ -1300,11 +1302,8 @@ g4_status g4_decoder_create(g4_ctx* ctx, const g4_decoder_desc* desc, const g4_d
 
 g4_status g4_decoder_destroy(g4_decoder* dec) {
     if (!dec) return G4_OK;
-    if (dec->ctx) {
-        cudaSetDevice(dec->ctx->device);
-        cudaStreamSynchronize(dec->ctx->stream);
-    }
-    for (void* p : dec->allocs) cudaFree(p);
+    cudaSetDevice(dec->device);
+    for (void* p : dec->allocs) cudaFree(p);  // waits for the device's work, this decoder's included
     delete dec;
     return G4_OK;
 }
@@ -1331,8 +1330,8 @@ g4_status g4_decoder_step(g4_ctx* ctx, g4_decoder* dec, const int32_t* ids, int3
     g4_status st = g4::use_device(ctx);
     if (st) return st;
     if (!dec || !ids || !seq_pos || !next) return g4::set_error(G4_ERR_INVALID, "g4_decoder_step: null argument");
-    if (dec->ctx->device != ctx->device)
-        return g4::set_error(G4_ERR_INVALID, "g4_decoder_step: decoder of device %d on device %d", dec->ctx->device,
+    if (dec->device != ctx->device)
+        return g4::set_error(G4_ERR_INVALID, "g4_decoder_step: decoder of device %d on device %d", dec->device,
                              ctx->device);
     DParams p = dec->p;
     p.ids = ids;

@@ -290,6 +290,7 @@ g4_status g4_dense_create(g4_ctx* ctx, const void* w_bf16, int K, int N, int src
         return g4::set_error(G4_ERR_UNSUPPORTED, "g4_dense_create: K=%d (multiple of 16) N=%d (multiple of 8)", K, N);
     g4_dense* d = new g4_dense();
     d->ctx = ctx;
+    d->device = ctx->device;
     d->K = K;
     d->N = N;
     const size_t bytes = (size_t)N * K * 2;
@@ -314,7 +315,7 @@ g4_status g4_dense_create(g4_ctx* ctx, const void* w_bf16, int K, int N, int src
 
 g4_status g4_dense_destroy(g4_dense* d) {
     if (!d) return G4_OK;
-    if (d->ctx) cudaSetDevice(d->ctx->device);
+    cudaSetDevice(d->device);
     cudaFree(d->w);
     delete d;
     return G4_OK;

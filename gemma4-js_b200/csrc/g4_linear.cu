@@ -438,6 +438,7 @@ g4_status g4_linear_create(g4_ctx* ctx, const void* packed_i32, const void* scal
         return g4::set_error(G4_ERR_UNSUPPORTED, "g4_linear_create: group size %d (only 32 is implemented)", group);
     g4_linear* lin = new g4_linear();
     lin->ctx = ctx;
+    lin->device = ctx->device;
     g4_linear_dev& L = lin->dev;
     L.K = K;
     L.N = N;
@@ -485,7 +486,7 @@ g4_status g4_linear_create(g4_ctx* ctx, const void* packed_i32, const void* scal
 
 g4_status g4_linear_destroy(g4_linear* lin) {
     if (!lin) return G4_OK;
-    if (lin->ctx) cudaSetDevice(lin->ctx->device);
+    cudaSetDevice(lin->device);
     cudaFree(lin->dev.wfrag);
     cudaFree(lin->dev.sfrag);
     cudaFree(lin->dev.tblk);

@@ -18,6 +18,7 @@ struct g4_linear_dev {
 
 struct g4_linear {
     g4_ctx* ctx = nullptr;
+    int device = 0;  // of ctx, which may be destroyed first
     g4_linear_dev dev;
 };
 

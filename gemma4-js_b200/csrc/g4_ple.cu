@@ -162,6 +162,7 @@ g4_status g4_ple_table_create(g4_ctx* ctx, const void* packed_u8, const void* sc
         return g4::set_error(G4_ERR_INVALID, "g4_ple_table_create: packed and scales must both be given or both NULL");
     g4_ple_table* t = new g4_ple_table();
     t->ctx = ctx;
+    t->device = ctx->device;
     t->vocab = vocab;
     t->width = width;
     t->group = group;
@@ -213,7 +214,7 @@ g4_status g4_ple_table_upload_rows(g4_ctx* ctx, g4_ple_table* tab, int row_start
 
 g4_status g4_ple_table_destroy(g4_ple_table* tab) {
     if (!tab) return G4_OK;
-    if (tab->ctx) cudaSetDevice(tab->ctx->device);
+    cudaSetDevice(tab->device);
     cudaFree(tab->packed);
     cudaFree(tab->scales);
     delete tab;
