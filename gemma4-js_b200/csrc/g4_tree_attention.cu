@@ -9,7 +9,9 @@
 // 128 rows per CTA (16 nodes of 8 heads).  Per tile and 128 rows that is 4 * 128 * 128 * hd
 // FLOP against 512 * hd B of K/V: 128 FLOP/B per CTA, so one CTA's worth of nodes is bound by
 // reading the cache (at 148 SMs even one node's 8 rows keep the tensor pipe ahead of HBM), and
-// four CTAs of one sequence (64 nodes) by the products.
+// four CTAs of one sequence (64 nodes) by the products.  Weights go to the second product as a
+// bf16 head and a bf16 tail, which makes it twice as long: 3072 clocks of tensor work per tile at
+// hd 256 instead of 2048.
 #include <algorithm>
 #include <type_traits>
 
@@ -28,8 +30,9 @@ constexpr int kRowsPerCta = 128;  // MMA M
 constexpr int kRest = 3 * 1024;   // shared memory besides Q and the ring
 // Four threads per query row, each with a quarter of a tile's keys (scores are read once and stay in
 // registers) and of O's columns: four warps per scheduler hide each other's latencies.  32 sequences
-// of 512 rows over 4160 keys at hd 256: 59.6 us, with two threads per row (scores read twice) 60.6; one
-// per row, a warp per scheduler, took 4500 clocks per tile instead of 2800.
+// of 512 rows over 4160 keys at hd 256 (before weights had tails, which take these 59.6 us to 71.1):
+// 59.6 us, with two threads per row (scores read twice) 60.6; one per row, a warp per scheduler, took
+// 4500 clocks per tile instead of 2800.
 constexpr int kParts = 4;
 constexpr int kSoftmaxWarps = 4 * kParts;
 constexpr int kKeysPerThread = kTile / kParts;
@@ -47,8 +50,11 @@ constexpr int kThreads = kSoftmaxThreads + 64;  // + TMA warp + MMA warp
 // rows of Q, S, P and O, but half of K's keys and half of V's columns, which the tensor cores of
 // both read: half the L2 and shared-memory traffic per row.  The even CTA issues every product;
 // commits arrive in both, and the odd one's MMA warp tells it when a granule has landed there.
-// Taken where a sequence has more than 128 rows: one sequence over a long cache at hd 512, whose
-// CTAs read K for 256 columns of V only, 83.7 us in single CTAs, 65.8 in pairs; hd 256, 61.7 and 60.6.
+// Taken at hd 256 and 512 where a sequence has more than 128 rows: one sequence over a long cache at
+// hd 512, whose CTAs read K for 256 columns of V only, 90.0 us in single CTAs, 73.5 in pairs; 32 x 64
+// nodes over 4160 keys 182 and 155, at hd 256 79.9 and 71.0.  At hd 128 the pair's longer chain of
+// arrivals costs more than its traffic saves (51.5 and 54.6 us; single CTAs are ahead in short and long
+// contexts, 23.2 and 27.2 us for 100 x 20 nodes over 500 keys).
 template <int HD, bool kPair>
 struct TreeCfg {
     static constexpr int HDV = HD < 256 ? HD : 256;           // O columns per CTA
@@ -57,7 +63,7 @@ struct TreeCfg {
     static constexpr int QBYTES = HD * 256;
     static constexpr int KKEYS = kPair ? kTile / 2 : kTile;    // of a tile's keys in this CTA's K
     static constexpr int VCOLS = kPair ? HDV / 2 : HDV;        // columns of this CTA's V
-    static constexpr int SLOT = HD == (kPair ? 128 : 64) ? 16384 : 32768;
+    static constexpr int SLOT = HD == 64 ? 16384 : 32768;
     static constexpr int KGRAN = HD * KKEYS * 2 / SLOT;        // granules per K tile
     static constexpr int KBOX = KKEYS * 128;                   // bytes of a K box
     static constexpr int KBOXES = SLOT / KBOX;                 // boxes per K granule
@@ -67,7 +73,7 @@ struct TreeCfg {
     static constexpr int SLOTS = SLOT == 16384 ? 8 : (229376 - QBYTES) / SLOT;
     static constexpr int SMEM = QBYTES + SLOTS * SLOT + kRest;  // the rest: TreeShared
     static_assert(SMEM <= 232448, "shared memory");
-    static_assert(!kPair || HD >= 128, "half of V is whole 64-column chunks");
+    static_assert(!kPair || HD >= 256, "pairs are for the wide heads");
 };
 
 struct TreeAttnParams {
@@ -224,9 +230,10 @@ __device__ __forceinline__ bool elect_one() {
     return e != 0;
 }
 constexpr uint32_t kTransposeB = 1u << 16;
-// Weights (bf16 pairs) lie over the scores they come from, each thread's over its own: TMEM column
-// of the 16-key step i.
+// Weights lie over the scores they come from, each thread's 32 over its own: 16 columns of heads (bf16
+// pairs), then 16 of tails.  TMEM column of the heads of the 16-key step i.
 __device__ __forceinline__ int p_col(int i) { return (i >> 1) * kKeysPerThread + (i & 1) * 8; }
+constexpr int kTail = kKeysPerThread / 2;
 // Floats (but NaN) in the order of integers, and back.
 __device__ __forceinline__ int ordered(int bits) { return bits < 0 ? bits ^ 0x7fffffff : bits; }
 constexpr int kLowest = (int)0x807fffff;  // ordered(-inf)
@@ -475,9 +482,11 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
                     if (elect_one()) {
                         const uint32_t b = va + slot * (C::SLOT >> 4), w = tmem + (t & 1) * 128;
 #pragma unroll
-                        for (int i = 0; i < C::VKEYS / 16; ++i)
-                            mma_ts<kPair>(o_tmem, w + p_col(a * (C::VKEYS / 16) + i), b + i * (2048 >> 4), pv_idesc,
-                                          (a | i) || t > 0 ? 1u : 0u);
+                        for (int i = 0; i < C::VKEYS / 16; ++i) {
+                            const uint32_t head = w + p_col(a * (C::VKEYS / 16) + i), bv = b + i * (2048 >> 4);
+                            mma_ts<kPair>(o_tmem, head, bv, pv_idesc, (a | i) || t > 0 ? 1u : 0u);
+                            mma_ts<kPair>(o_tmem, head + kTail, bv, pv_idesc, 1u);
+                        }
                         commit_to<kPair>(&sh.empty[slot]);
                         if (a == C::VGRAN - 1) commit_to<kPair>(&sh.o_done[t & 1]);
                     }
@@ -595,19 +604,24 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
                         tmem_st_32x32b_x32(o_part + c, o);
                     }
                 }
-                // P in bf16 (the product's operand type; at most 1 part in 256 per weight) over the
-                // scores just read; l sums the rounded weights, so they are weights of sum 1.
-                uint32_t w[16];
+                // P as a bf16 head and a bf16 tail (the product's operand type): 2^-16 of a weight is lost,
+                // as in g4_attention_rows, so that verifying a token and decoding it differ by no more than
+                // the order of their sums.  In heads alone a weight loses 2^-9, which is as much again as the
+                // rounding of the result (2.2e-3 of its norm instead of 1.65e-3).
+                uint32_t w[32];
                 float l0 = 0.f, l1 = 0.f;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     const float a = ex2(fmaf(__uint_as_float(x[2 * i]), kLog2e, -mu));
                     const float b = ex2(fmaf(__uint_as_float(x[2 * i + 1]), kLog2e, -mu));
+                    l0 += a;
+                    l1 += b;
                     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[i]) : "f"(b), "f"(a));
-                    l0 += __uint_as_float(w[i] << 16);
-                    l1 += __uint_as_float(w[i] & 0xffff0000u);
+                    asm("cvt.rn.bf16x2.f32 %0, %1, %2;"
+                        : "=r"(w[kTail + i])
+                        : "f"(b - __uint_as_float(w[i] & 0xffff0000u)), "f"(a - __uint_as_float(w[i] << 16)));
                 }
-                tmem_st_32x32b_x16(s_tmem + (t & 1) * 128, w);
+                tmem_st_32x32b_x32(s_tmem + (t & 1) * 128, w);
                 l += l0 + l1;
                 tmem_st_wait();
             }
@@ -818,11 +832,11 @@ g4_status launch_tree_attention_t(g4_ctx* ctx, const g4_kv* kv, TreeAttnParams p
     const long long ctas = (long long)across * p.nseq;
     // Split the keys while that adds CTAs to SMs without one: down to one tile per split up to 16
     // splits (which the join reads in one round trip), then to two.  One sequence of 8 nodes over 4096
-    // keys: 14.1 us at one tile, 13.6 at two, 14.3 at three; 8 sequences with a window of 512 (five
-    // tiles): 12.9, 16.7 and 18.0.  A split costs a start, a drain, the join and the partial rows'
-    // way to L2 and back, so it has to save four tiles: 64 sequences of 16 nodes with a window of 512
-    // take 33.5 us in two splits (two tiles saved), 19.7 whole, 32 of them 23.6 in four (three saved)
-    // and 19.0, 16 of them 16.9 in five (four saved) and 18.9.
+    // keys: 14.8 us at one tile, 14.6 so, 15.3 at two, 15.6 at three; 8 sequences with a window of 512
+    // (five tiles): 15.2, 17.7 and 19.6 at one, two and three.  A split costs a start, a drain, the join
+    // and the partial rows' way to L2 and back, so it has to save four tiles: 64 sequences of 16 nodes
+    // with a window of 512 take 35.5 us in two splits (two tiles saved), 22.1 whole, 32 of them 24.4 in
+    // three (three saved) and 21.4, 16 of them 17.5 in five (four saved) and 21.2.
     int nsplit = (int)std::max<long long>(
         1, std::min<long long>({ctx->num_sms / ctas, std::max(ntiles / 2, std::min(ntiles, 16)), kMaxSplits}));
     if (ntiles - (ntiles + nsplit - 1) / nsplit < 4) nsplit = 1;
@@ -857,7 +871,7 @@ g4_status launch_tree_attention_t(g4_ctx* ctx, const g4_kv* kv, TreeAttnParams p
 }
 template <int HD>
 g4_status launch_tree_attention(g4_ctx* ctx, const g4_kv* kv, const TreeAttnParams& p) {
-    if constexpr (HD >= 128) {
+    if constexpr (HD >= 256) {
         if (p.tree.nodes * p.heads > kRowsPerCta) return launch_tree_attention_t<HD, true>(ctx, kv, p);
     }
     return launch_tree_attention_t<HD, false>(ctx, kv, p);
@@ -882,7 +896,7 @@ g4_status tree_maps(g4_kv* kv) {
 template <int HD>
 g4_status tree_maps_all(g4_kv* kv) {
     g4_status st = tree_maps<HD, false>(kv);
-    if constexpr (HD >= 128) {
+    if constexpr (HD >= 256) {
         if (!st) st = tree_maps<HD, true>(kv);
     }
     return st;

@@ -552,8 +552,10 @@ class Gemma4Model:
         `sampling`), the path whose drafted tokens equal those picks is accepted, its K/V rows are
         moved together and the positions advanced by its length.  Returns device tensors: picks
         [B, n], path [B, n] (-1 behind it), accepted [B] and next [B] (also in buf["next"]), the
-        pick after the path.  Greedy picks give the tokens of as many decode steps; sampled ones
-        their distribution, since each accepted token is the sample drawn at its node."""
+        pick after the path.  Greedy picks give the tokens of as many decode steps but for near ties
+        (the attention of both weighs to 2^-16, in sums of another order; above 16 rows a step the
+        linears are the batched ones); sampled ones their distribution, since each accepted token is
+        the sample drawn at its node."""
         B, n = tokens.shape
         rows = B * n
         if B > self.max_batch or rows > self.max_rows:

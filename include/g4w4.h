@@ -406,7 +406,8 @@ typedef struct {
  * Row (s, i) sees the cached keys j < base and, of the drafted ones, its ancestors and itself;
  * when sliding, only keys less than `window` positions before its own (a drafted key's position
  * is base + its depth).  q, out: bf16 [rows, heads, hd], rows a multiple of nodes; logit scale
- * 1.0; heads 1..8, hd in {64,128,256,512}, q and out 16-byte aligned.  What masked cache rows
+ * 1.0; heads 1..8, hd in {64,128,256,512}, q and out 16-byte aligned.  Weights are kept to 2^-16,
+ * as in g4_attention_rows, sums in f32.  What masked cache rows
  * hold, NaN and infinity included, does not reach a row that does not see them; a row that sees
  * a value (V) that is not finite is NaN throughout (at hd 512: in the value's half of the
  * columns).  A sequence whose drafted rows would
