@@ -555,16 +555,22 @@ class Gemma4Model:
         pick after the path.  Greedy picks give the tokens of as many decode steps but for near ties
         (the attention of both weighs to 2^-16, in sums of another order; above 16 rows a step the
         linears are the batched ones); sampled ones their distribution, since each accepted token is
-        the sample drawn at its node."""
+        the sample drawn at its node.
+
+        Of a tree that reaches past max_seq the first nodes that fit are used (a node's parent is one of
+        them), as if counts said so: at the last position node 0 alone, and a full sequence sits the step
+        out, like one of count 0 (accepted 0, its next as it was)."""
         B, n = tokens.shape
         rows = B * n
         if B > self.max_batch or rows > self.max_rows:
             raise G4Error(-1, f"verify_step: {B} trees of {n} nodes (max_batch {self.max_batch}, max_rows {self.max_rows})")
         if tokens.dtype != torch.int32 or not tokens.is_contiguous() or tokens.device != self.dev:
             raise G4Error(-1, f"verify_step: tokens must be a contiguous int32 tensor on {self.dev}")
+        self.ops._tree("verify_step", parents, B, n, counts)
+        given, counts = counts, self._fitting(B, n, counts)
         tree = self.ops._tree("verify_step", parents, B, n, counts)
         picks = self._tree_buffer("picks", rows, torch.int32)
-        if counts is not None:  # unused nodes: any valid token, their rows are not looked at
+        if given is not None:  # unused nodes: any valid token, their rows are not looked at
             self.buf["ids"][:rows].copy_(tokens.reshape(-1).clamp(0, self.cfg.vocab - 1))
         else:
             self.buf["ids"][:rows].copy_(tokens.reshape(-1))
@@ -577,8 +583,13 @@ class Gemma4Model:
         path, accepted, nxt = self.ops.treeAccept(parents, tokens, picks, counts)
         kv_compact(self.ctx, self._own_caches(), self.seq_pos, path, accepted, seq_stride=self.max_seq)
         call("g4_advance_positions_each", self.ctx.handle, _ptr(self.seq_pos), 0, B, _ptr(accepted))
-        self.buf["next"][:B].copy_(nxt if counts is None else torch.where(accepted > 0, nxt, self.buf["next"][:B]))
+        self.buf["next"][:B].copy_(torch.where(accepted > 0, nxt, self.buf["next"][:B]))
         return {"picks": picks, "path": path, "accepted": accepted, "next": self.buf["next"][:B]}
+
+    def _fitting(self, B: int, n: int, counts: torch.Tensor | None) -> torch.Tensor:
+        """Nodes of each tree that are used: those asked for, as far as their positions exist."""
+        free = (self.max_seq - self.seq_pos[:B]).clamp_(min=0)
+        return free.clamp_(max=n) if counts is None else torch.minimum(counts, free)
 
     def _tree_buffer(self, name: str, n: int, dtype) -> torch.Tensor:
         t = self.buf.get("tree_" + name)
