@@ -352,6 +352,7 @@ class Gemma4Model:
         self._alloc(self.max_rows)
         self.graph = None
         self._capturing = False
+        self._outgrown = []
         self.ops = GPUOps(ctx)
 
     def _cache(self, spec: dict, ring_kv: bool) -> KVCache:
@@ -592,8 +593,13 @@ class Gemma4Model:
         return free.clamp_(max=n) if counts is None else torch.minimum(counts, free)
 
     def _tree_buffer(self, name: str, n: int, dtype) -> torch.Tensor:
+        """A verify step's buffer of n or more entries, grow-only.  An outgrown one is kept (a captured step
+        may use it), and each is at least twice the one before: all of them take no more than the last."""
         t = self.buf.get("tree_" + name)
         if t is None or t.numel() < n:
+            if t is not None:
+                self._outgrown.append(t)
+                n = max(n, 2 * t.numel())
             t = self.buf["tree_" + name] = torch.zeros(n, dtype=dtype, device=self.dev)
         return t
 
