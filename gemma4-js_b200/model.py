@@ -615,7 +615,8 @@ class Gemma4Model:
 
     def capture_decode(self, batch: int | None = None, sampling: Sampling | None = None):
         """Captures one decode step (next <- argmax(model(next)), or the sampled pick with the
-        numbers that sampling.uniform holds at each replay) in a CUDA graph."""
+        numbers that sampling.uniform holds at each replay) in a CUDA graph.  The graph keeps the tensors
+        of `sampling`: to change a setting, write into them."""
         B = batch or self.max_batch
         saved = self.buf["next"][:B].clone()
         self.decode_step(batch=B, sampling=sampling)  # warm-up: sizes workspaces and sets kernel attributes
@@ -638,6 +639,7 @@ class Gemma4Model:
         self.ctx.set_stream(old)
         self.graph_kernels = launch_count() - n0   # libg4w4 kernels per replayed step
         self.graph, self.graph_stream, self.graph_batch = g, stream, B
+        g.sampling = None if sampling is None else replace(sampling)  # the tensors, whatever becomes of the caller's object
         return g
 
     def replay_decode(self):

@@ -1,5 +1,8 @@
-"""Captured steps replayed after other calls of the same model."""
+"""Captured steps replayed after other calls of the same model, and after the caller dropped what it
+captured them with."""
+import gc
 import importlib
+import weakref
 
 import numpy as np
 import pytest
@@ -9,6 +12,42 @@ from test_drafted_model_gpu import W_KW, build, greedy_run, small_cfg
 
 pytestmark = pytest.mark.gpu
 model = importlib.import_module("gemma4-js_b200.model")
+
+
+def test_a_captured_sampled_step_keeps_its_settings(rt):
+    cfg = small_cfg()
+    w = model.random_weights(cfg, seed=43, **W_KW)
+    B, steps = 2, 5
+    u = torch.rand((steps, B), generator=torch.Generator().manual_seed(1))
+
+    def run(drop):
+        m = build(rt, rt.Context(0), cfg, w, B)
+        for s in range(B):
+            m.buf["next"][s] = m.prefill(s, [3 + s, 2, 1])
+        uniform = torch.zeros(B, device="cuda")
+        sm = model.Sampling(uniform=uniform, temperature=torch.full((B,), 0.7, device="cuda"),
+                            top_k=torch.full((B,), 60, dtype=torch.int32, device="cuda"))
+        m.capture_decode(batch=B, sampling=sm)
+        kept = [weakref.ref(sm.temperature), weakref.ref(sm.top_k)]
+        g = m.graph
+        if drop:  # the caller keeps graph and random numbers, lets go of the rest, and memory is used again
+            sm.temperature = sm.top_k = None
+            del sm
+            m.capture_decode(batch=1)  # another graph of the model takes the first one's place in it
+            gc.collect()
+            assert all(r() is not None for r in kept)
+            junk = [torch.full((64,), 1e9, device="cuda") for _ in range(200)]  # noqa: F841
+        out = []
+        for i in range(steps):
+            uniform.copy_(u[i])
+            torch.cuda.synchronize()
+            g.replay()
+            torch.cuda.synchronize()
+            out.append(m.buf["next"][:B].tolist())
+        m.ctx.check_device()
+        return out
+
+    assert run(True) == run(False)
 
 
 def test_a_captured_verify_step_survives_a_larger_one(rt):
