@@ -288,13 +288,14 @@ class Sampling:
     top_p: torch.Tensor | None = None
     min_p: torch.Tensor | None = None
 
-    def struct(self, rows: int) -> G4Sampling:
+    def struct(self, rows: int, device: torch.device) -> G4Sampling:
         p = []
         for name in ("temperature", "top_k", "top_p", "min_p", "uniform"):
             t = getattr(self, name)
             want = torch.int32 if name == "top_k" else torch.float32
-            if t is not None and (t.dtype != want or not t.is_cuda or not t.is_contiguous() or t.numel() < rows):
-                raise G4Error(-1, f"sampling: {name} must be a contiguous {want} device tensor of {rows} rows")
+            if t is not None and (t.dtype != want or t.device != device or not t.is_contiguous() or t.numel() < rows):
+                raise G4Error(-1, f"sampling: {name} must be a contiguous {want} tensor of {rows} rows on {device}, got "
+                                  f"{t.dtype} of {t.numel()} on {t.device}")
             p.append(None if t is None else t.data_ptr())
         return G4Sampling(*p)
 
@@ -477,7 +478,7 @@ class Gemma4Model:
         """logits + greedy (gemma4-webgpu.js:413-480), or g4_sample of the capped logits."""
         cfg, h = self.cfg, self.ctx.handle
         if sampling is not None:
-            how = sampling.struct(rows)
+            how = sampling.struct(rows, self.ctx.torch_device)
             call("g4_dense_matmul", h, self.head.handle, _ptr(xh), rows, _ptr(logits))
             call("g4_sample", h, _ptr(logits), cfg.vocab, rows, cfg.vocab, C.c_float(cfg.softcap), C.byref(how), _ptr(ids),
                  _ptr(vals))
