@@ -79,11 +79,18 @@ class Context:
         before the context stream is done with them."""
         if torch._C._cuda_getCurrentRawStream(self.device) == self._raw_stream:
             return torch.empty(shape, dtype=dtype, device=self.torch_device)
-        for t in used:
-            if t is not None:
-                t.record_stream(self._stream)
+        self.use(*used)
         with torch.cuda.stream(self._stream):
             return torch.empty(shape, dtype=dtype, device=self.torch_device)
+
+    def use(self, *tensors: torch.Tensor | None) -> None:
+        """The context stream is going to read or write these: when it is not torch's current stream, their
+        memory is not handed out again before it is done with them."""
+        if torch._C._cuda_getCurrentRawStream(self.device) == self._raw_stream:
+            return
+        for t in tensors:
+            if t is not None:
+                t.record_stream(self._stream)
 
     def empty_like(self, t: torch.Tensor, dtype: torch.dtype, *used: torch.Tensor | None) -> torch.Tensor:
         """empty() in the shape of a contiguous t (which torch makes in half the time)."""
@@ -310,6 +317,7 @@ def kv_compact(ctx: Context, caches, seq_pos: torch.Tensor, path: torch.Tensor, 
     sp = _need(ctx, "kv_compact", "seq_pos", seq_pos, torch.int32)
     if seq_base < 0 or seq_base + nseq > seq_pos.numel():
         raise G4Error(-6, f"kv_compact: sequences {seq_base}..{seq_base + nseq} of {seq_pos.numel()} positions")
+    ctx.use(seq_pos, path, accepted)
     call("g4_kv_compact", ctx.handle, _cache_table(caches), len(caches), _seq_stride(caches, seq_stride), sp, seq_base,
          nseq, nodes, pp, ap)
 
@@ -324,6 +332,7 @@ def kv_fork(ctx: Context, caches, seq_pos: torch.Tensor, src, dst, seq_stride: i
     n = len(src)
     if any(not 0 <= i < seq_pos.numel() for i in (*src, *dst)):
         raise G4Error(-6, f"kv_fork: sequences {src} -> {dst} of {seq_pos.numel()} positions")
+    ctx.use(seq_pos)
     call("g4_kv_fork", ctx.handle, _cache_table(caches), len(caches), _seq_stride(caches, seq_stride), sp,
          (C.c_int32 * n)(*src), (C.c_int32 * n)(*dst), n)
 
@@ -509,7 +518,10 @@ class GPUOps:
             out = self.ctx.empty_like(q, torch.bfloat16, seq_pos, parents, counts)
             if counts is not None:  # rows that no node writes
                 self.ctx.fill(out, 0)
-        op = _need(self.ctx, "attentionTree", "out", out, torch.bfloat16, q.shape)
+            op = out.data_ptr()
+        else:
+            op = _need(self.ctx, "attentionTree", "out", out, torch.bfloat16, q.shape)
+            self.ctx.use(q, seq_pos, parents, counts, out)
         rmap = G4Rows(sp, seq_base, nodes, 0, 0)
         call("g4_attention_tree", self.ctx.handle, qp, cache.handle, nseq * nodes, heads, hd, C.byref(rmap),
              C.byref(tree), cache.seq_rows if cache.ring else _seq_stride([cache], seq_stride), int(bool(sliding)), window,
