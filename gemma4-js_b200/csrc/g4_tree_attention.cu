@@ -78,6 +78,7 @@ struct TreeCfg {
 
 struct TreeAttnParams {
     const uint16_t* q;
+    const uint16_t* v;  // the cache's values (its tensor map's)
     uint16_t* out;
     float* part_o;   // [nsplit][nseq * nodes * heads][HD] (nsplit > 1)
     float2* part_ml; // [nsplit][HD / HDV][nseq * nodes * heads]: running maximum (base 2), sum
@@ -88,12 +89,17 @@ struct TreeAttnParams {
     int krows, vrows;  // rows of the tensor maps' boxes (the whole granule, or a part in ring caches)
 };
 
+// Tiles that not every row sees whole: the drafted rows lie in one or two, and the rows' windows start
+// less than 64 keys apart, the first of them at the first key of the first tile.
+constexpr int kMasked = 3;
 struct TreeShared {
     uint64_t full[8], empty[8];
     uint64_t peer_full[8];  // pairs: the granule has landed in the odd CTA
     uint64_t q_full, s_full[2], p_ready[2], o_done[2], v_full, scanned, drained;
     uint32_t tmem;
-    uint32_t poison[3][4];  // keys of a masked tile whose V row is not finite (three tiles in turn)
+    uint32_t poison[kMasked][4];  // keys of each masked tile whose V row is not finite
+    int masked_key[kMasked];      // and its first key
+    uint32_t poisoned;            // whether there are any
     int parents[G4_TREE_MAX_NODES];
     int mx[3][kRowsPerCta];  // a row's maximum, ordered as integers (three tiles in turn)
 };
@@ -517,7 +523,8 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
             if (!good && (int)threadIdx.x < count) raise_error(p.err, G4_DEVERR_BAD_INDEX);
             sh.parents[threadIdx.x] = good ? parent : -1;
         }
-        if (threadIdx.x < 4) sh.poison[0][threadIdx.x] = 0u;
+        if (threadIdx.x < kMasked * 4) sh.poison[threadIdx.x >> 2][threadIdx.x & 3] = 0u;
+        if (threadIdx.x == 0) sh.poisoned = 0u;
         const int rows = count * p.heads;              // of this sequence
         asm volatile("cp.async.wait_all;" ::: "memory");
         fence_proxy_async_smem();
@@ -626,12 +633,12 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
                 tmem_st_wait();
             }
             if (masked) {
-                // What no row sees must not reach the product: 0 * NaN.  Thread = key and a part of the
+                // What a row does not see must not reach its product: 0 * NaN.  Thread = key and a part of the
                 // columns: rows behind base + count become 0; values that are not finite become 0 and
-                // are remembered.
+                // are remembered, for the rows that see them.
                 const int key = threadIdx.x & 127, vrow = key % C::VKEYS, g = v_granule(t) + key / C::VKEYS;
-                uint32_t* poison = sh.poison[nmasked % 3];
-                if (threadIdx.x < 4) sh.poison[(nmasked + 1) % 3][threadIdx.x] = 0u;  // last read two masked tiles ago
+                uint32_t* poison = sh.poison[nmasked];
+                if (threadIdx.x == 0) sh.masked_key[nmasked] = k0;
                 ok = ok && wait_on<false>(&sh.v_full, nmasked & 1, p.err, 712);
                 ok = ok && wait_on<false>(&sh.full[g % C::SLOTS], (g / C::SLOTS) & 1, p.err, 713);  // of this phase now
                 ++nmasked;
@@ -665,7 +672,11 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
                     }
                     if (bad) {
                         atomicOr(&poison[key >> 5], 1u << lane);
-                        if (kPair) or_in(&poison[key >> 5], rank ^ 1, 1u << lane);  // its rows see the same keys
+                        sh.poisoned = 1u;
+                        if (kPair) {  // its rows see the same keys
+                            or_in(&poison[key >> 5], rank ^ 1, 1u << lane);
+                            or_in(&sh.poisoned, rank ^ 1, 1u);
+                        }
                     }
                     fence_proxy_async_smem();
                 }
@@ -679,9 +690,6 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
                 } else {
                     softmax_sync();
                 }
-#pragma unroll 1
-                for (int w = 0; w < 4; ++w)
-                    if (poison[w] & visible(k0, w)) l = __int_as_float(0x7fffffff);  // sees a V row that is not finite
             }
             tc_fence_before();
             tell(&sh.p_ready[t & 1]);
@@ -701,6 +709,33 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
             }
         }
         tc_fence_after();
+        if (nt > 0 && warp_live && ok && has_o && sh.poisoned) {
+            // What was taken out of V comes back into its column of the rows that see it, as if the product
+            // had met it.
+            const size_t row0 = (size_t)(p.seq_base + s) * p.seq_stride;
+            const uint16_t* v = p.v + row0 * HD + vhalf * C::HDV + part * C::OCOLS;
+#pragma unroll 1
+            for (int c = 0; c < C::OCOLS; c += 32) {
+                uint32_t o[32];
+                tmem_ld_32x32b_x32(o_part + c, o);
+                tmem_ld_wait(o);
+#pragma unroll 1
+                for (int w = 0; w < nmasked * 4; ++w) {
+                    const int k0 = sh.masked_key[w >> 2];
+                    for (uint32_t bits = sh.poison[w >> 2][w & 3] & visible(k0, w & 3); bits; bits &= bits - 1) {
+                        const int key = k0 + 32 * (w & 3) + __ffs(bits) - 1;
+                        const uint16_t* e = v + (size_t)(p.ring ? key % p.ring : key) * HD + c;
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            if ((e[i] & 0x7f80u) == 0x7f80u)
+                                o[i] = __float_as_uint(__uint_as_float(o[i]) + __uint_as_float((uint32_t)e[i] << 16));
+                    }
+                }
+                __syncwarp();
+                tmem_st_32x32b_x32(o_part + c, o);
+            }
+            tmem_st_wait();
+        }
         // Rows leave through shared memory: written
         // by row, 16-byte chunks permuted within 128 B against bank conflicts, read back along the
         // rows, so that global stores are whole lines.  (Stores from the row's own thread touch 32
@@ -944,7 +979,7 @@ extern "C" g4_status g4_attention_tree(g4_ctx* ctx, const void* q_bf16, const g4
         return g4::set_error(G4_ERR_RANGE, "g4_attention_tree: sequences beyond the cache (%d rows)", kv->rows_total);
     st = g4::check_ring("g4_attention_tree", kv, sliding, window, tree->nodes);
     if (st) return st;
-    const TreeAttnParams p{static_cast<const uint16_t*>(q_bf16), static_cast<uint16_t*>(out_bf16), nullptr, nullptr,
+    const TreeAttnParams p{static_cast<const uint16_t*>(q_bf16), kv->v, static_cast<uint16_t*>(out_bf16), nullptr, nullptr,
                            ctx->d_err, *tree, map->seq_pos, map->seq_base, map->pos0, seq_stride, heads,
                            sliding ? 1 : 0, window, kv->ring, kv->ring ? kv->capacity : seq_stride, 1, nseq,
                            (map->flags & G4_ROWS_HISTORY_READY) ? 1 : 0};

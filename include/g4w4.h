@@ -407,11 +407,10 @@ typedef struct {
  * when sliding, only keys less than `window` positions before its own (a drafted key's position
  * is base + its depth).  q, out: bf16 [rows, heads, hd], rows a multiple of nodes; logit scale
  * 1.0; heads 1..8, hd in {64,128,256,512}, q and out 16-byte aligned.  Weights are kept to 2^-16,
- * as in g4_attention_rows, sums in f32.  What masked cache rows
- * hold, NaN and infinity included, does not reach a row that does not see them; a row that sees
- * a value (V) that is not finite is NaN throughout (at hd 512: in the value's half of the
- * columns).  A sequence whose drafted rows would
- * not fit its seq_stride (or a ring cache's capacity) is left out and raises
+ * as in g4_attention_rows, sums in f32.  What masked cache rows hold, NaN and infinity included,
+ * does not reach a row that does not see them; a value (V) that is not finite leaves the rows that
+ * see it not finite (NaN or infinite) in its column, and no other element.  A sequence whose drafted
+ * rows would not fit its seq_stride (or a ring cache's capacity) is left out and raises
  * G4_DEVERR_BAD_INDEX.  Long key ranges are split over CTAs with partial results in the context
  * workspace (as g4_attention_rows).  G4_ROWS_HISTORY_READY as for g4_attention_rows. */
 g4_status g4_attention_tree(g4_ctx* ctx, const void* q_bf16, const g4_kv* kv, int rows, int heads, int hd,
