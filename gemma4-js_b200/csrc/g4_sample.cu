@@ -974,7 +974,7 @@ constexpr int kWideWarps = kWide / 32;
 constexpr int kParts = 8192;
 constexpr int kList = 8192;
 constexpr int kSegment = 512;      // at most kWide segments per CTA
-constexpr int kFixed = 44;         // bits of a listed weight: kList of them stay below 2^58
+constexpr int kFixed = 50;         // bits of a listed weight: kList of them reach 2^63, and lose 2^-37 of the highest in all
 constexpr int kCount = 256;      // listed logits ranked by counting
 
 struct NucleusShared {
