@@ -1369,7 +1369,9 @@ __global__ void __launch_bounds__(kWide, 1) sample_nucleus_kernel(const SamplePa
                 const double z = __shfl_up_sync(0xffffffffu, upto, o);
                 if (lane >= o) upto += z;
             }
-            double at = S.start + (upto - own), bw = 0.0;
+            double left = __shfl_up_sync(0xffffffffu, upto, 1);  // (upto - own would be 0 beside a much larger own)
+            if (lane == 0) left = 0.0;
+            double at = S.start + left, bw = 0.0;
             int best = -1;
 #pragma unroll 4
             for (int k = 0; k < 16; ++k) {
@@ -1851,7 +1853,9 @@ struct General {
                 const double z = __shfl_up_sync(0xffffffffu, y, q);
                 if (lane >= q) y += z;
             }
-            double at = run + (y - s);
+            double left = __shfl_up_sync(0xffffffffu, y, 1);  // (y - s would be 0 beside a much larger s)
+            if (lane == 0) left = 0.0;
+            double at = run + left;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 if (x[e] > 0.0 && at <= target) best = i0 + e, bw = x[e];
