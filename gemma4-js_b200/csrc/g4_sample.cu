@@ -1252,7 +1252,7 @@ __global__ void __launch_bounds__(kWide, 1) sample_nucleus_kernel(const SamplePa
             unsigned long long past = 0;  // what the listed above those to rank weigh
             int left = n;
             if (n > kCount) {
-                // 512 parts of even width again: what is listed in the one where the prefix ends is ranked.
+                // 1024 parts of even width again: what is listed in the one where the prefix ends is ranked.
                 const float from = (float)((double)a + (double)b0 * part), fine = (float)kWide * scale / (float)(b1 + 1 - b0);
                 auto fine_of = [&](unsigned long long f) {
                     return max(0, min(kWide - 1, (int)((key_logit((uint32_t)(f >> 32)) - from) * fine)));

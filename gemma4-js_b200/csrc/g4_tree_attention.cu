@@ -51,10 +51,10 @@ constexpr int kThreads = kSoftmaxThreads + 64;  // + TMA warp + MMA warp
 // both read: half the L2 and shared-memory traffic per row.  The even CTA issues every product;
 // commits arrive in both, and the odd one's MMA warp tells it when a granule has landed there.
 // Taken at hd 256 and 512 where a sequence has more than 128 rows: one sequence over a long cache at
-// hd 512, whose CTAs read K for 256 columns of V only, 90.0 us in single CTAs, 73.5 in pairs; 32 x 64
-// nodes over 4160 keys 182 and 155, at hd 256 79.9 and 71.0.  At hd 128 the pair's longer chain of
-// arrivals costs more than its traffic saves (51.5 and 54.6 us; single CTAs are ahead in short and long
-// contexts, 23.2 and 27.2 us for 100 x 20 nodes over 500 keys).
+// hd 512, whose CTAs read K for 256 columns of V only, 90.4 us in single CTAs, 75.2 in pairs; 32 x 64
+// nodes over 4160 keys 184 and 156, at hd 256 79.5 and 71.1 (100 x 20 nodes over 500 keys, where start
+// and drain count: 31.0 and 35.0).  At hd 128 the pair's longer chain of arrivals costs more than its
+// traffic saves: 51.2 and 53.5 us, in the short contexts 22.5 and 26.0.
 template <int HD, bool kPair>
 struct TreeCfg {
     static constexpr int HDV = HD < 256 ? HD : 256;           // O columns per CTA
@@ -867,11 +867,11 @@ g4_status launch_tree_attention_t(g4_ctx* ctx, const g4_kv* kv, TreeAttnParams p
     const long long ctas = (long long)across * p.nseq;
     // Split the keys while that adds CTAs to SMs without one: down to one tile per split up to 16
     // splits (which the join reads in one round trip), then to two.  One sequence of 8 nodes over 4096
-    // keys: 14.8 us at one tile, 14.6 so, 15.3 at two, 15.6 at three; 8 sequences with a window of 512
-    // (five tiles): 15.2, 17.7 and 19.6 at one, two and three.  A split costs a start, a drain, the join
+    // keys: 14.3 us at one tile, 14.2 so, 15.0 at two, 15.2 at three; 8 sequences with a window of 512
+    // (five tiles): 14.8, 16.9 and 18.9 at one, two and three.  A split costs a start, a drain, the join
     // and the partial rows' way to L2 and back, so it has to save four tiles: 64 sequences of 16 nodes
-    // with a window of 512 take 35.5 us in two splits (two tiles saved), 22.1 whole, 32 of them 24.4 in
-    // three (three saved) and 21.4, 16 of them 17.5 in five (four saved) and 21.2.
+    // with a window of 512 take 34.8 us in two splits (two tiles saved), 21.1 whole, 32 of them 23.5 in
+    // three (three saved) and 20.1, 16 of them 17.1 in five (four saved) and 20.1.
     int nsplit = (int)std::max<long long>(
         1, std::min<long long>({ctx->num_sms / ctas, std::max(ntiles / 2, std::min(ntiles, 16)), kMaxSplits}));
     if (ntiles - (ntiles + nsplit - 1) / nsplit < 4) nsplit = 1;

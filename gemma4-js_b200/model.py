@@ -553,11 +553,13 @@ class Gemma4Model:
         node, the model's pick after each node is taken (greedy, or sampled by row b * n + i of
         `sampling`), the path whose drafted tokens equal those picks is accepted, its K/V rows are
         moved together and the positions advanced by its length.  Returns device tensors: picks
-        [B, n], path [B, n] (-1 behind it), accepted [B] and next [B] (also in buf["next"]), the
-        pick after the path.  Greedy picks give the tokens of as many decode steps but for near ties
-        (the attention of both weighs to 2^-16, in sums of another order; above 16 rows a step the
-        linears are the batched ones); sampled ones their distribution, since each accepted token is
-        the sample drawn at its node.
+        [B, n], path [B, n] (-1 behind it), accepted [B] and next [B], the pick after the path.
+        picks and next are the model's own buffers (next is buf["next"]): the next step writes them.
+
+        Greedy picks give the tokens of as many decode steps but for near ties (the attention of both
+        weighs to 2^-16, in sums of another order; above 16 rows a step the linears are the batched
+        ones); sampled ones their distribution, since each accepted token is the sample drawn at its
+        node.
 
         Of a tree that reaches past max_seq the first nodes that fit are used (a node's parent is one of
         them), as if counts said so: at the last position node 0 alone, and a full sequence sits the step
