@@ -288,12 +288,14 @@ class Sampling:
     top_p: torch.Tensor | None = None
     min_p: torch.Tensor | None = None
 
-    def struct(self, rows: int, device: torch.device) -> G4Sampling:
+    def struct(self, rows: int, device: torch.device | None = None) -> G4Sampling:
+        """The settings of `rows` rows for a call on `device` (default: the GPU of `uniform`)."""
         p = []
+        device = device or self.uniform.device
         for name in ("temperature", "top_k", "top_p", "min_p", "uniform"):
             t = getattr(self, name)
             want = torch.int32 if name == "top_k" else torch.float32
-            if t is not None and (t.dtype != want or t.device != device or not t.is_contiguous() or t.numel() < rows):
+            if t is not None and (t.dtype != want or not t.is_cuda or t.device != device or not t.is_contiguous() or t.numel() < rows):
                 raise G4Error(-1, f"sampling: {name} must be a contiguous {want} tensor of {rows} rows on {device}, got "
                                   f"{t.dtype} of {t.numel()} on {t.device}")
             p.append(None if t is None else t.data_ptr())

@@ -379,7 +379,7 @@ typedef struct {
  * ids_out[r] is the lowest index i whose kept weights up to and with i, in index order, sum to
  * more than uniform[r] times the kept weight; probs_out[r] (may be NULL) its share of the kept
  * weight (1 for a greedy row).  A row with nothing to pick gives -1 and 0.  Weights and sums
- * are held in 64 bits (weights to 2e-14; below 2^-1021 of the highest they count as 0); the same
+ * are held in 64 bits (weights to 2e-14; below some 2^-1021 of the highest they count as 0); the same
  * call gives the same bits.
  * vocab at most 786432 (G4_ERR_UNSUPPORTED). */
 g4_status g4_sample(g4_ctx* ctx, const float* logits, long long ld, int rows, int vocab, float cap,

@@ -27,12 +27,17 @@ class Tensor:
 def test_settings_of_another_gpu_are_refused():
     here = torch.device("cuda", 0)
     s = model.Sampling(uniform=Tensor("cuda:0"), temperature=Tensor("cuda:0"), top_k=Tensor("cuda:0", torch.int32))
-    assert s.struct(4, here).uniform == 4096
+    assert s.struct(4, here).uniform == 4096 and s.struct(4).temperature == 4096
     for name in ("uniform", "temperature", "top_k", "top_p", "min_p"):
         bad = model.Sampling(uniform=Tensor("cuda:0"))
         setattr(bad, name, Tensor("cuda:1", torch.int32 if name == "top_k" else torch.float32))
         with pytest.raises(rt.G4Error, match=name):
             bad.struct(4, here)
+        if name != "uniform":
+            with pytest.raises(rt.G4Error, match=name):
+                bad.struct(4)
     for bad in (Tensor("cuda:0", n=3), Tensor("cuda:0", torch.float64), torch.zeros(4)):
         with pytest.raises(rt.G4Error, match="uniform"):
             model.Sampling(uniform=bad).struct(4, here)
+        with pytest.raises(rt.G4Error, match="uniform"):
+            model.Sampling(uniform=bad).struct(4)
