@@ -10,8 +10,8 @@
 // FLOP against 512 * hd B of K/V: 128 FLOP/B per CTA, so one CTA's worth of nodes is bound by
 // reading the cache (at 148 SMs even one node's 8 rows keep the tensor pipe ahead of HBM), and
 // four CTAs of one sequence (64 nodes) by the products.  Weights go to the second product as a
-// bf16 head and a bf16 tail, which makes it twice as long: 3072 clocks of tensor work per tile at
-// hd 256 instead of 2048.
+// bf16 head and a bf16 tail, which makes it twice as long: half as much tensor work again as the
+// 2048 clocks per tile at hd 256.
 #include <algorithm>
 #include <type_traits>
 
