@@ -613,7 +613,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
                 }
                 // P as a bf16 head and a bf16 tail (the product's operand type): 2^-16 of a weight is lost,
                 // as in g4_attention_rows, so that verifying a token and decoding it differ by no more than
-                // the order of their sums.  In heads alone a weight loses 2^-9, which is as much again as the
+                // the order of their sums.  In heads alone a weight loses 2^-8, which is as much again as the
                 // rounding of the result (2.2e-3 of its norm instead of 1.65e-3).
                 uint32_t w[32];
                 float l0 = 0.f, l1 = 0.f;
